@@ -11,12 +11,13 @@ STATUS_NONFINITE_CODE = 0x1
 STATUS_BAD_SCALE = 0x2
 STATUS_WAIT_TIMEOUT = 0x4
 STATUS_NONFINITE_INPUT = 0x8
+STATUS_BAD_INDEX = 0x10
 OUT_F32 = 0
 OUT_BF16 = 1
 SCHEDULE_FRESH_WEIGHT = 0x100
 
 _c = ctypes
-_i64, _ptr, _int, _sz = _c.c_int64, _c.c_void_p, _c.c_int, _c.c_size_t
+_i64, _ptr, _int, _sz, _f32 = _c.c_int64, _c.c_void_p, _c.c_int, _c.c_size_t, _c.c_float
 
 # name -> (restype, argtypes); must list every symbol include/bfp8.h declares
 SIGNATURES = {
@@ -57,6 +58,14 @@ SIGNATURES = {
     "bfp8_swiglu_interleave_weight": (_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _ptr]),
     "bfp8_gemm_block128_swiglu": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64,
                                          _i64, _i64, _i64, _ptr, _sz, _ptr, _ptr]),
+    "bfp8_moe_route_workspace_bytes": (_sz, [_i64, _i64]),
+    "bfp8_moe_route": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _int, _int, _f32, _ptr, _ptr, _ptr, _sz,
+                              _ptr]),
+    "bfp8_moe_block128_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "bfp8_moe_block128": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
+                                 _int, _ptr, _sz, _ptr, _ptr, _int, _i64]),
+    "bfp8_moe_layer_block128": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _int, _int, _f32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                       _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _int, _ptr, _sz, _ptr, _ptr]),
 }
 
 _lib = None

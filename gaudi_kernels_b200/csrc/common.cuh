@@ -68,6 +68,9 @@ int sm_count();
 int make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
                        uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                        CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
+// `outer` contiguous byte matrices [mid, inner]; a box is one matrix deep.
+int make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t mid, uint64_t outer,
+                       uint32_t box_inner, uint32_t box_mid, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
 // One flag per device ordinal, shared by the host threads that call into the library.
 typedef std::atomic<bool> DeviceFlags[64];

@@ -488,17 +488,14 @@ EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
-// 2-D row-major tensor map; box_inner * element size must not exceed the swizzle span (128 bytes by default).
-int make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
-                       uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
+// Encodes a tiled tensor map of one-element strides.
+static int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
+                             const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return BFP8_ERR_CUDA;
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_stride_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
   auto encode = [&] {
-    return fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+    return fn(map, dt, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
@@ -514,6 +511,24 @@ int make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* bas
     return BFP8_ERR_CUDA;
   }
   return BFP8_OK;
+}
+
+// 2-D row-major tensor map; box_inner * element size must not exceed the swizzle span (128 bytes by default).
+int make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
+                       uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[2] = {inner, outer};
+  const cuuint64_t strides[1] = {row_stride_bytes};
+  const cuuint32_t box[2] = {box_inner, box_outer};
+  return encode_tensor_map(map, dt, 2, base, dims, strides, box, swizzle);
+}
+
+// `outer` contiguous matrices [mid, inner] of bytes; a box is one matrix deep and clipped at that matrix's own edges.
+int make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t mid, uint64_t outer,
+                       uint32_t box_inner, uint32_t box_mid, CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[3] = {inner, mid, outer};
+  const cuuint64_t strides[2] = {inner, inner * mid};
+  const cuuint32_t box[3] = {box_inner, box_mid, 1};
+  return encode_tensor_map(map, dt, 3, base, dims, strides, box, swizzle);
 }
 
 // CTAs per tile of the split form (1: no split), priced with what B200 measured: a K block takes 0.48 us, a launch that

@@ -45,6 +45,8 @@ extern "C" {
 #define BFP8_STATUS_WAIT_TIMEOUT   0x4u  /* a bounded barrier wait inside a kernel gave up */
 #define BFP8_STATUS_NONFINITE_INPUT 0x8u /* an activation was inf or NaN */
 
+#define BFP8_STATUS_BAD_INDEX      0x10u /* an expert index was beyond the last expert */
+
 #define BFP8_OUT_F32  0
 #define BFP8_OUT_BF16 1
 
@@ -326,6 +328,53 @@ int bfp8_peer_close(void* ptr);
  * BFP8_STATUS_WAIT_TIMEOUT is raised in *status_dev and the kernel returns.  Each rank must run on its own GPU. */
 int bfp8_peer_barrier(uint32_t* const* flags, int rank, int world_size, uint32_t epoch,
                       int64_t wait_limit_cycles, uint32_t* status_dev, void* stream);
+
+/* Router of a mixture-of-experts layer: the top_k experts of every token and their weights.
+ *   l[t, e] = fp32(sum_c x[t, c] * router[e, c])          (the sum is held to about 1e-8 of its terms' size)
+ *   BFP8_ROUTE_SOFTMAX  the largest l; weights softmax(l) at them (over the chosen ones alone with renormalize)
+ *   BFP8_ROUTE_SIGMOID  s = fp32(sigmoid(l)); the largest fp32(s + bias) (bias may be NULL); weights s at them (divided
+ *                       by their sum + 1e-20 with renormalize)
+ * and all weights times `scale`.  Choices come in descending order, ties by the lower index; a NaN ranks last.
+ *   x bf16 [t, h] (row stride ldx), router bf16 [experts, h] (row stride ld_router), bias fp32 [experts]
+ *   ids int32 [t, top_k], weights fp32 [t, top_k], contiguous
+ * top_k <= 32, experts <= 512 (BFP8_ERR_UNSUPPORTED beyond, and for a bias with softmax).  workspace:
+ * bfp8_moe_route_workspace_bytes(t, experts) bytes, 4-byte aligned, in any state.  The reference has no counterpart. */
+#define BFP8_ROUTE_SOFTMAX 0
+#define BFP8_ROUTE_SIGMOID 1
+size_t bfp8_moe_route_workspace_bytes(int64_t t, int64_t experts);
+int bfp8_moe_route(const uint16_t* x, int64_t ldx, const uint16_t* router, int64_t ld_router, const float* bias,
+                   int64_t t, int64_t h, int64_t experts, int64_t top_k, int scoring, int renormalize, float scale,
+                   int32_t* ids, float* weights, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Routed experts of a few tokens, block-scaled E4M3 weights:
+ *   xq = x quantized as bfp8_quant_act_1x128_bf16 does (a group that holds an inf or NaN becomes NaN)
+ *   h[s] = silu(xq[t] . Wgate[id]^T) * (xq[t] . Wup[id]^T)   of slot s = (t, j), id = ids[t, j], in fp32
+ *   hq = h quantized by the same rule;   out[t] = bf16(sum_j weights[t, j] * (hq[t, j] . Wdown[id]^T))
+ *   w_gate_up E4M3 [experts, 2, inter, h] (gate, then up), s_gate_up fp32 [experts, 2, ceil(inter/128), ceil(h/128)]
+ *   w_down    E4M3 [experts, h, inter],                    s_down    fp32 [experts, ceil(h/128), ceil(inter/128)]
+ *   ids int32 [t, top_k]: a negative one adds nothing (an expert of another GPU); one beyond the last expert adds
+ *   nothing either and raises BFP8_STATUS_BAD_INDEX.  An expert may occur several times in a token.
+ *   out bf16 [t, h], row stride ldo (ldo % 4 == 0, 8-byte aligned); x bf16 [t, h], row stride ldx
+ * t <= 128, top_k <= 32, t * top_k <= 2048, experts <= 512, h and inter multiples of 16 (BFP8_ERR_UNSUPPORTED otherwise);
+ * weights 16-byte aligned and contiguous.  workspace: bfp8_moe_block128_workspace_bytes() bytes, 256-byte aligned, in any
+ * state; calls that may overlap on the device need separate ones.  The second kernel is launched cooperatively on all
+ * SMs.  max_ctas / wait_limit_cycles: as bfp8_gemm_block128_ex.  status |= WAIT_TIMEOUT if an internal wait gave up; the
+ * output is then undefined.  Sums are formed in a fixed order: results repeat bit for bit for the same ids.  The reference
+ * has no counterpart. */
+size_t bfp8_moe_block128_workspace_bytes(int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t inter);
+int bfp8_moe_block128(const uint16_t* x, int64_t ldx, const int32_t* ids, const float* weights,
+                      const uint8_t* w_gate_up, const float* s_gate_up, const uint8_t* w_down, const float* s_down,
+                      uint16_t* out, int64_t ldo, int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t inter,
+                      int native_half, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream,
+                      int max_ctas, int64_t wait_limit_cycles);
+
+/* bfp8_moe_route followed by bfp8_moe_block128 on its choice, in two kernels: ids and weights (both written) are those
+ * bfp8_moe_route gives, out has the bits of the two calls. */
+int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* router, int64_t ld_router, const float* bias,
+                            int scoring, int renormalize, float scale, int32_t* ids, float* weights,
+                            const uint8_t* w_gate_up, const float* s_gate_up, const uint8_t* w_down, const float* s_down,
+                            uint16_t* out, int64_t ldo, int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t inter,
+                            int native_half, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
 
 #ifdef __cplusplus
 }
