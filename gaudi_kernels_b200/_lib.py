@@ -58,6 +58,9 @@ SIGNATURES = {
     "bfp8_swiglu_interleave_weight": (_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _ptr]),
     "bfp8_gemm_block128_swiglu": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64,
                                          _i64, _i64, _i64, _ptr, _sz, _ptr, _ptr]),
+    "bfp8_gemm_group_w4": (_int, [_ptr, _i64, _int, _ptr, _ptr, _ptr, _int, _ptr, _ptr, _int, _i64, _i64, _i64, _i64, _ptr,
+                                  _ptr, _i64]),
+    "bfp8_quant_group_w4_f32": (_int, [_ptr, _i64, _i64, _i64, _int, _ptr, _ptr, _ptr, _int, _ptr]),
     "bfp8_moe_route_workspace_bytes": (_sz, [_i64, _i64]),
     "bfp8_moe_route": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _int, _int, _f32, _ptr, _ptr, _ptr, _sz,
                               _ptr]),

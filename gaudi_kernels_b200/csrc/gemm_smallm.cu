@@ -760,6 +760,8 @@ int smallm_cluster_size(int64_t tiles, int64_t groups, int sms) {
 // anything still in flight (bfp8_set_weights_at_rest).
 static std::atomic<int> g_weights_at_rest{0};
 
+bool weights_at_rest() { return g_weights_at_rest.load(std::memory_order_relaxed) != 0; }
+
 int set_weights_at_rest(int on) { return g_weights_at_rest.exchange(on != 0 ? 1 : 0, std::memory_order_relaxed); }
 
 int launch_gemm_smallm(const uint8_t* a_codes, int64_t lda, const float* a_scales, int64_t ldsa,

@@ -1,0 +1,525 @@
+// Products of a few activation rows with a 4-bit weight (sm_100a):
+//   out[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group] (+ bias[n]),   group 32, 64 or 128.
+//
+// A few rows read the weight once: the call is bound by HBM, N K / 2 bytes, as long as the 4-bit values can be turned into
+// operands fast enough - at 6.5 TB/s every SM has to unpack about 50 of them per cycle.  So:
+//   * 16 weight rows x 16 k are the A operand of mma.sync (m16n8k16) and 8 activation rows the B operand, with A formed in
+//     registers: a 32-bit word holds 8 consecutive k of one row; (w & 0x000f000f) | magic is a pair of 16-bit floats 128 + q
+//     (1024 + q in fp16), and one fused multiply-add per pair subtracts 128 + z.  q - z is exact, so the tensor core sees
+//     the exact integers, sums of a group are formed in fp32, and the scale multiplies the group's fp32 sum.  tcgen05 would
+//     need the unpacked operand in shared memory, four times the bytes that come from HBM.
+//   * which k a thread's operand register stands for is free as long as A and B agree: a thread owns 8 consecutive k of each
+//     32, the word as it lies in memory, and pairs (k, k + 4) of x by byte permutes.
+//   * the weight streams through a ring of shared-memory stages, 256 k of the CTA's rows each, by TMA; x comes with it.
+//     Scales and zero points go from global memory to registers one stage ahead and are handed round by shuffles.
+//   * a CTA has R rows (a multiple of 16) and a slice of K: R and the cluster size are chosen so that the CTAs fill the SMs
+//     once with the least per CTA (w4_plan).  Inside the CTA the warps split R and, where that leaves warps over, the
+//     stages; the CTAs of a cluster add their sums through distributed shared memory.  All sums in a fixed order.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace bfp8 {
+
+bool weights_at_rest();
+
+namespace {
+
+constexpr long long kDefaultWaitLimit = 2000000000LL;      // about a second
+constexpr int kStageK = 256;                               // k per stage: 128 bytes of a code row
+constexpr int kMaxRows = 256;                              // weight rows per CTA, the largest TMA box
+constexpr int kMaxStages = 16;
+constexpr int kRingBytes = 208 * 1024;
+constexpr int kMaxCluster = 8;
+
+struct W4Params {
+  const uint16_t* scales;      // [n, groups]
+  const uint8_t* zeros;        // [n, groups] or NULL: 8
+  const float* bias;           // [n] or NULL
+  void* out;
+  int64_t ldo;
+  int m, n, k, groups;
+  int rows;                    // R
+  int slices;                  // warps that share a row range: they take the stages in turn
+  int stages;                  // ring depth, a multiple of slices: the stage a warp waits for is one it has emptied itself, so
+                               // the phase it waits for cannot be mistaken for an older one of the same parity
+  int cluster;
+  int out_f32;
+  int w_early;
+  long long wait_limit;
+  uint32_t* status;
+};
+
+struct W4Tail {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint32_t abort_flag;
+};
+
+template <bool kBf16>
+struct Half16;
+template <>
+struct Half16<true> {
+  static constexpr uint32_t kMagic = 0x43004300u, kOne = 0x3f803f80u, kSixteenth = 0u, kStep = 0u, kMinus = 0xc300c300u;
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+  }
+  static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits << 16); }
+  static __device__ __forceinline__ uint16_t round(float v) { return static_cast<uint16_t>(float_to_bf16_bits(v)); }
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Half16<false> {
+  static constexpr uint32_t kMagic = 0x64006400u, kOne = 0x3c003c00u, kSixteenth = 0x2c002c00u, kMinus = 0xe400e400u;
+  static constexpr uint32_t kStep = 0x63806380u;           // 960 = 1024 - 64
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+  }
+  static __device__ __forceinline__ float value(uint32_t bits) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  }
+  static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+// (w & mask) | magic in one instruction
+__device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+  return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// kNT: activation rows / 8; kMT: 16-row weight tiles per warp (x is read from shared memory once for all of them);
+// kShift: group = 32 << kShift.
+// Warps that multiply; with the producer the sums of 32 rows x 64 weight rows fit in the registers of eight warps.
+__host__ __device__ constexpr int consumers(int nt) { return nt >= 4 ? 7 : 15; }
+
+template <bool kBf16, int kNT, int kMT, int kShift>
+__global__ void __launch_bounds__((consumers(kNT) + 1) * 32, 1)
+w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Params p) {
+  using H = Half16<kBf16>;
+  constexpr int kConsumers = consumers(kNT), kThreads = (kConsumers + 1) * 32;
+  constexpr int kMp = kNT * 8;
+  constexpr int kXBytes = kMp * kStageK * 2;
+  constexpr int kStageGroups = kStageK >> (5 + kShift);            // scale groups per stage: 8, 4, 2
+  constexpr int kHeld = kStageGroups / 2;                          // registers of scales per 16-row tile and stage
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + kRingBytes);
+  volatile uint32_t* abort_flag = &tail->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = p.rows / (16 * kMT);                           // warps across R
+  const int slices = p.slices;
+  const uint32_t stage_bytes = static_cast<uint32_t>(p.rows) * 128u + kXBytes;
+  const int rank = p.cluster > 1 ? static_cast<int>(blockIdx.x) % p.cluster : 0;
+  const int n0 = static_cast<int>(blockIdx.x) / p.cluster * p.rows;
+  const int m0 = blockIdx.y * kMp;
+  const int all_steps = (p.k + kStageK - 1) / kStageK;
+  const int step0 = static_cast<int>(static_cast<long long>(all_steps) * rank / p.cluster);
+  const int step1 = static_cast<int>(static_cast<long long>(all_steps) * (rank + 1) / p.cluster);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&tail->full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), static_cast<uint32_t>(units));
+    }
+    tail->abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  ptx::griddep_launch_dependents();
+
+  float acc[kMT][kNT][4];
+#pragma unroll
+  for (int a = 0; a < kMT; ++a)
+#pragma unroll
+    for (int b = 0; b < kNT; ++b)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[a][b][c] = 0.0f;
+  const int unit = warp % units, slice = warp / units;
+
+  if (warp == kConsumers) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      ptx::prefetch_tensormap(&tmap_w);
+      ptx::prefetch_tensormap(&tmap_x);
+      const uint64_t once = ptx::l2_policy_evict_first();
+      int early = 0;
+      if (p.w_early)                                               // codes at rest: asked for before the previous kernel has ended
+        for (; early < p.stages && step0 + early < step1; ++early) {
+          const uint32_t full = ptx::smem_u32(&tail->full[early]);
+          ptx::mbar_arrive_expect_tx(full, stage_bytes);
+          ptx::tma_load_2d_hint(smem_base + early * stage_bytes, &tmap_w, full, (step0 + early) * 128, n0, once);
+        }
+      ptx::griddep_wait();
+      uint32_t stage = 0, parity = 0;
+      for (int s = step0; s < step1; ++s) {
+        const uint32_t full = ptx::smem_u32(&tail->full[stage]), dst = smem_base + stage * stage_bytes;
+        if (early > 0) {
+          --early;
+        } else {
+          if (!ptx::mbar_wait(ptx::smem_u32(&tail->empty[stage]), parity ^ 1u, abort_flag, p.wait_limit)) break;
+          ptx::mbar_arrive_expect_tx(full, stage_bytes);
+          ptx::tma_load_2d_hint(dst, &tmap_w, full, s * 128, n0, once);
+        }
+#pragma unroll
+        for (int b = 0; b < kStageK / 64; ++b)
+          ptx::tma_load_2d(dst + p.rows * 128 + b * kMp * 128, &tmap_x, full, s * kStageK + b * 64, m0);
+        if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; parity ^= 1u; }
+      }
+    }
+  } else if (slice < slices) {
+    // ------------------------------------------------------------------ consumers
+    ptx::griddep_wait();
+    const int g = lane >> 2, t = lane & 3;
+    // activation row of column g of the B operand: neighbouring columns lie in different halves of the swizzled 128 bytes
+    const int xrow = (g >> 1) + 4 * (g & 1);
+    // scale and zero point of (row lane & 15 of tile a, group 2 r + lane / 16 of step s) in one register
+    uint32_t held[kMT][kHeld];
+    auto fetch = [&](int s) {
+#pragma unroll
+      for (int a = 0; a < kMT; ++a)
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+          const int row = n0 + (unit * kMT + a) * 16 + (lane & 15), gr = s * kStageGroups + 2 * r + (lane >> 4);
+          uint32_t v = 0u;
+          if (row < p.n && gr < p.groups) {
+            const int64_t at = static_cast<int64_t>(row) * p.groups + gr;
+            v = __ldg(p.scales + at) | ((p.zeros != nullptr ? static_cast<uint32_t>(__ldg(p.zeros + at)) : 8u) << 16);
+          }
+          held[a][r] = v;
+        }
+    };
+    if (step0 + slice < step1) fetch(step0 + slice);
+    int stage = slice, parity = 0;
+    for (int s = step0 + slice; s < step1; s += slices) {
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit))) break;
+      const uint32_t wbase = smem_base + stage * stage_bytes + unit * kMT * 2048 + g * 128 + t * 4;
+      const uint32_t xbase = smem_base + stage * stage_bytes + p.rows * 128 + xrow * 128;
+      uint32_t now[kMT][kHeld];
+#pragma unroll
+      for (int a = 0; a < kMT; ++a)
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) now[a][r] = held[a][r];
+      if (s + slices < step1) fetch(s + slices);
+      float part[kMT][kNT][4];
+      uint32_t sub0[kMT][2], sub1[kMT][2];
+      float scale[kMT][2];
+#pragma unroll
+      for (int q = 0; q < kStageK / 32; ++q) {
+        constexpr int kMask = (1 << kShift) - 1;
+        if ((q & kMask) == 0) {                                    // a new group
+          const int gr = q >> kShift;
+#pragma unroll
+          for (int a = 0; a < kMT; ++a) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t v = __shfl_sync(0xffffffffu, now[a][gr >> 1], (gr & 1) * 16 + g + 8 * r);
+              scale[a][r] = H::value(v & 0xffffu);
+              sub0[a][r] = H::kMinus + (v >> 16) * 0x10001u;       // -(128 + z), fp16 -(1024 + z), in both halves
+              if (!kBf16) sub1[a][r] = H::fma(sub0[a][r], H::kOne, H::kStep);      // -(64 + z)
+            }
+#pragma unroll
+            for (int b = 0; b < kNT; ++b)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) part[a][b][c] = 0.0f;
+          }
+        }
+        uint32_t x[kNT][4];
+#pragma unroll
+        for (int b = 0; b < kNT; ++b) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (m0 + b * 8 + xrow < p.m)
+            v = lds128(xbase + (q >> 1) * (kMp * 128) + b * 1024 + ((((q & 1) * 4 + t) ^ xrow) << 4));
+          x[b][0] = __byte_perm(v.x, v.z, 0x5410);                 // (k, k + 4) for k = 0 .. 3
+          x[b][1] = __byte_perm(v.x, v.z, 0x7632);
+          x[b][2] = __byte_perm(v.y, v.w, 0x5410);
+          x[b][3] = __byte_perm(v.y, v.w, 0x7632);
+        }
+#pragma unroll
+        for (int a = 0; a < kMT; ++a) {
+          uint32_t w[2][4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t lo = lds32(wbase + a * 2048 + r * 1024 + ((q ^ g) << 4)), hi = lo >> 8;
+            w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+            w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+            if (kBf16) {                                           // seven bits of fraction: no room for a value shifted by four
+              w[r][1] = H::fma(pick(lo >> 4, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+              w[r][3] = H::fma(pick(lo >> 12, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+            } else {                                               // 1024 + 16 q, times 1/16
+              w[r][1] = H::fma(pick(lo, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
+              w[r][3] = H::fma(pick(hi, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < kNT; ++b) {
+            H::mma(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1]);
+            H::mma(part[a][b], w[0][2], w[1][2], w[0][3], w[1][3], x[b][2], x[b][3]);
+          }
+          if ((q & kMask) == kMask)
+#pragma unroll
+            for (int b = 0; b < kNT; ++b)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc[a][b][c] = fmaf(part[a][b][c], scale[a][c >> 1], acc[a][b][c]);
+        }
+      }
+      __syncwarp();
+      ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->empty[stage]), lane);
+      stage += slices;
+      if (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
+    }
+  }
+
+  // ------------------------------------------------------------------ sums of the slices, then of the cluster's CTAs
+  __syncthreads();                                                 // every stage has been read: the ring is free
+  float* red = reinterpret_cast<float*>(smem);                     // [slice][activation row][weight row]
+  const int width = units * 16 * kMT;
+  if (warp < kConsumers && slice < slices) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int a = 0; a < kMT; ++a)
+#pragma unroll
+      for (int b = 0; b < kNT; ++b)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          red[(slice * kMp + b * 8 + t + 4 * (c & 1)) * width + (unit * kMT + a) * 16 + g + 8 * (c >> 1)] = acc[a][b][c];
+  }
+  __syncthreads();
+  const bool whole = *abort_flag == 0;
+  const int count = min(kMp, p.m - m0) * width;
+  if (p.cluster > 1) {
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+      float v = red[i];
+      for (int s = 1; s < slices; ++s) v += red[s * kMp * width + i];
+      red[i] = v;
+    }
+    ptx::cluster_sync_all();
+  }
+  auto store = [&](int i, float v) {
+    const int m = i / width, n = n0 + i - m * width;
+    if (i - m * width >= p.rows || n >= p.n) return;
+    if (p.bias != nullptr) v += __ldg(p.bias + n);
+    const int64_t at = static_cast<int64_t>(m0 + m) * p.ldo + n;
+    if (p.out_f32) static_cast<float*>(p.out)[at] = v;
+    else static_cast<uint16_t*>(p.out)[at] = H::round(v);
+  };
+  if (p.cluster > 1) {
+    // CTA `rank` finishes its share of the outputs, adding the CTAs' sums in rank order, which is K order
+    const int i1 = static_cast<int>(static_cast<long long>(count) * (rank + 1) / p.cluster);
+    for (int i = static_cast<int>(static_cast<long long>(count) * rank / p.cluster) + threadIdx.x; i < i1 && whole; i += kThreads) {
+      float v = 0.0f;
+      for (int c = 0; c < p.cluster; ++c) v += ld_cluster_f32(ptx::cluster_map(smem_base + i * 4, c));
+      store(i, v);
+    }
+    ptx::cluster_sync_all();                                       // nobody leaves while its sums are being read
+  } else if (whole) {
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+      float v = red[i];
+      for (int s = 1; s < slices; ++s) v += red[s * kMp * width + i];
+      store(i, v);
+    }
+  }
+  ptx::idle_after_abort(abort_flag);
+  if (threadIdx.x == 0 && tail->abort_flag != 0) atomicOr(p.status, BFP8_STATUS_WAIT_TIMEOUT);
+}
+
+// Rows per CTA and CTAs per cluster: the fewest bytes for the CTA that has most of them.  A cluster's exchange costs about
+// as much time as a CTA needs for 32 KB.  step: the rows that one warp handles.
+struct Plan {
+  int rows, cluster;
+};
+Plan w4_plan(int64_t n, int64_t k, int step, int warps, int sms) {
+  const int most = step * warps < kMaxRows ? step * warps : kMaxRows;
+  const int64_t steps = (k + kStageK - 1) / kStageK;
+  Plan best = {step, 1};
+  int64_t best_cost = INT64_MAX;
+  for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2) {
+    if (cluster > steps) break;
+    for (int rows = step; rows <= most; rows += step) {
+      const int64_t tiles = (n + rows - 1) / rows, waves = (tiles * cluster + sms - 1) / sms;
+      const int64_t cost = waves * (rows * 128 * ((steps + cluster - 1) / cluster) + 4096) + (cluster > 1 ? 32768 : 0);
+      if (cost < best_cost) { best_cost = cost; best = {rows, cluster}; }
+    }
+  }
+  return best;
+}
+
+template <bool kBf16, int kNT, int kMT, int kShift>
+int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
+  constexpr int smem = 1024 + kRingBytes + static_cast<int>(sizeof(W4Tail));
+  static_assert(smem <= 227 * 1024, "shared memory of one SM");
+  auto kernel = w4_kernel<kBf16, kNT, kMT, kShift>;
+  static DeviceFlags done;
+  int rc = ensure_smem_limit(kernel, smem, done);
+  if (rc != BFP8_OK) return rc;
+  const Plan plan = w4_plan(p.n, p.k, 16 * kMT, consumers(kNT), sm_count());
+  p.rows = plan.rows;
+  p.cluster = plan.cluster;
+  const int stage_bytes = p.rows * 128 + kNT * 8 * kStageK * 2;
+  const int most = kRingBytes / stage_bytes < kMaxStages ? kRingBytes / stage_bytes : kMaxStages;
+  p.slices = consumers(kNT) / (p.rows / (16 * kMT));
+  if (p.slices > most) p.slices = most;
+  p.stages = most / p.slices * p.slices;
+  alignas(64) CUtensorMap tmap_w, tmap_x;
+  rc = make_tensor_map_2d(&tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, p.k / 2, p.n, p.k / 2, 128, p.rows);
+  if (rc != BFP8_OK) return rc;
+  rc = make_tensor_map_2d(&tmap_x, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, p.k, p.m,
+                          ldx * 2, 64, kNT * 8);
+  if (rc != BFP8_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>((p.m + kNT * 8 - 1) / (kNT * 8)), 1);
+  cfg.blockDim = dim3((consumers(kNT) + 1) * 32, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+  BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmap_w, tmap_x, p));
+  return BFP8_OK;
+}
+
+template <bool kBf16, int kNT, int kMT>
+int launch_group(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
+  if (group == 32) return launch_w4<kBf16, kNT, kMT, 0>(codes, x, ldx, p, st);
+  if (group == 64) return launch_w4<kBf16, kNT, kMT, 1>(codes, x, ldx, p, st);
+  return launch_w4<kBf16, kNT, kMT, 2>(codes, x, ldx, p, st);
+}
+
+template <bool kBf16>
+int launch_rows(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
+  if (p.m <= 8) return launch_group<kBf16, 1, 1>(group, codes, x, ldx, p, st);
+  if (p.m <= 16) return launch_group<kBf16, 2, 2>(group, codes, x, ldx, p, st);
+  return launch_group<kBf16, 4, 4>(group, codes, x, ldx, p, st);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Quantizer: one warp per group of a row
+// ---------------------------------------------------------------------------------------------------------------------
+template <bool kBf16>
+__device__ __forceinline__ float rounded16(float v) { return Half16<kBf16>::value(Half16<kBf16>::round(v)); }
+
+// zeros != NULL: s = rounded((max(max w, 0) - min(min w, 0)) / 15), z = clamp(rne(-min / s), 0, 15); otherwise
+// s = rounded(max|w| / 7), z = 8.  q = clamp(rne(w / s) + z, 0, 15).  A group of zeros gets s = 1.
+template <bool kBf16>
+__global__ void __launch_bounds__(256)
+quant_group_w4_kernel(const float* __restrict__ w, int64_t n, int k, int64_t ldw, int group, int groups,
+                      uint8_t* __restrict__ codes, uint16_t* __restrict__ scales, uint8_t* __restrict__ zeros) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (item >= n * groups) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = item / groups;
+  const int k0 = static_cast<int>(item - row * groups) * group, len = min(group, k - k0);
+  const float* src = w + row * ldw + k0;
+  float lo = 0.0f, hi = 0.0f;
+  for (int c = lane; c < len; c += 32) {
+    const float v = src[c];
+    lo = fminf(lo, v);
+    hi = fmaxf(hi, v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  float s = rounded16<kBf16>(zeros != nullptr ? __fdiv_rn(hi - lo, 15.0f) : __fdiv_rn(fmaxf(hi, -lo), 7.0f));
+  if (s == 0.0f) s = 1.0f;
+  const int z = zeros != nullptr ? static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.0f), 15.0f)) : 8;
+  if (lane == 0) {
+    scales[item] = Half16<kBf16>::round(s);
+    if (zeros != nullptr) zeros[item] = static_cast<uint8_t>(z);
+  }
+  auto code = [&](int c) {
+    const float q = rintf(__fdiv_rn(src[c], s)) + static_cast<float>(z);
+    return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(q, 0.0f), 15.0f)));
+  };
+  for (int c = 2 * lane; c < len; c += 64)                         // k % 32 == 0: pairs are whole
+    codes[row * (k / 2) + (k0 + c) / 2] = static_cast<uint8_t>(code(c) | (code(c + 1) << 4));
+}
+
+}  // namespace
+}  // namespace bfp8
+
+using namespace bfp8;
+
+extern "C" int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const uint8_t* codes, const uint16_t* scales,
+                                  const uint8_t* zeros, int group, const float* bias, void* out, int out_f32, int64_t ldo,
+                                  int64_t m, int64_t n, int64_t k, uint32_t* status_dev, void* stream, int64_t wait_limit_cycles) {
+  if (!x || !codes || !scales || !out || !status_dev) return BFP8_ERR_NULL;
+  if (m <= 0 || n <= 0 || k <= 0 || m > (1 << 20) || n > (1 << 30) || k > (1 << 30) || ldx < k || ldo < n) return BFP8_ERR_SHAPE;
+  if (x_dtype != BFP8_W4_BF16 && x_dtype != BFP8_W4_F16) return BFP8_ERR_SHAPE;
+  if (group != 32 && group != 64 && group != 128) return BFP8_ERR_UNSUPPORTED;
+  if (k % 32 != 0) return BFP8_ERR_UNSUPPORTED;
+  if (!aligned(x, 16) || ldx % 8 != 0 || !aligned(codes, 16) || !aligned(scales, 2) || !aligned(out, out_f32 ? 4 : 2) ||
+      (bias && !aligned(bias, 4)) || !aligned(status_dev, 4))
+    return BFP8_ERR_ALIGN;
+  W4Params p = {};
+  p.scales = scales;
+  p.zeros = zeros;
+  p.bias = bias;
+  p.out = out;
+  p.ldo = ldo;
+  p.m = static_cast<int>(m);
+  p.n = static_cast<int>(n);
+  p.k = static_cast<int>(k);
+  p.groups = static_cast<int>((k + group - 1) / group);
+  p.out_f32 = out_f32 != 0;
+  p.w_early = weights_at_rest() ? 1 : 0;
+  p.wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kDefaultWaitLimit;
+  p.status = status_dev;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return x_dtype == BFP8_W4_BF16 ? launch_rows<true>(group, codes, x, ldx, p, st) : launch_rows<false>(group, codes, x, ldx, p, st);
+}
+
+extern "C" int bfp8_quant_group_w4_f32(const float* w, int64_t n, int64_t k, int64_t ldw, int group, uint8_t* codes,
+                                       uint16_t* scales, uint8_t* zeros, int scale_dtype, void* stream) {
+  if (!w || !codes || !scales) return BFP8_ERR_NULL;
+  if (n <= 0 || k <= 0 || n > (1 << 30) || k > (1 << 30) || ldw < k) return BFP8_ERR_SHAPE;
+  if (scale_dtype != BFP8_W4_BF16 && scale_dtype != BFP8_W4_F16) return BFP8_ERR_SHAPE;
+  if ((group != 32 && group != 64 && group != 128) || k % 32 != 0) return BFP8_ERR_UNSUPPORTED;
+  if (!aligned(w, 4) || !aligned(scales, 2)) return BFP8_ERR_ALIGN;
+  const int64_t groups = (k + group - 1) / group, blocks = (n * groups + 7) / 8;
+  if (blocks > 2147483647LL) return BFP8_ERR_SHAPE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+  if (scale_dtype == BFP8_W4_BF16)
+    quant_group_w4_kernel<true><<<grid, block, 0, st>>>(w, n, static_cast<int>(k), ldw, group, static_cast<int>(groups), codes, scales, zeros);
+  else
+    quant_group_w4_kernel<false><<<grid, block, 0, st>>>(w, n, static_cast<int>(k), ldw, group, static_cast<int>(groups), codes, scales, zeros);
+  BFP8_CUDA_TRY(cudaGetLastError());
+  return BFP8_OK;
+}

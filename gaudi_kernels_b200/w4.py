@@ -1,0 +1,104 @@
+"""4-bit weights with a scale (and a zero point) per group of k, for products of a few activation rows.
+
+W[n, k] = (q[n, k] - z[n, k // group]) * s[n, k // group], q packed two to a byte (even k in the low four bits).  The weight is
+read as it is stored: no repacked copy.  Kernels: libbfp8.so, csrc/w4.cu.  The reference has no 4-bit weights.
+"""
+
+import torch
+
+from . import _lib
+from .block_fp8_gemm import _WAIT_TIMEOUT_MSG
+from .fp8_codec import _device_for, _device_guard, _empty, _read_status, _status_buffer, _stream_ptr, _unread_status_buffer
+
+GROUPS = (32, 64, 128)
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def quantize_group_w4(w, group=128, zeros=True, scale_dtype=torch.bfloat16):
+    """fp32 [N, K] -> (codes uint8 [N, K / 2], scales [N, ceil(K / group)], zeros uint8 of that shape or None).
+
+    With zeros: s = round((max(w, 0) - min(w, 0)) / 15), z = clamp(rne(-min / s), 0, 15); without: s = round(max|w| / 7) and
+    z = 8 everywhere.  q = clamp(rne(w / s) + z, 0, 15).  Scales are rounded to scale_dtype (bfloat16 or float16) before they
+    are used.  K is a multiple of 32.
+    """
+    if not isinstance(w, torch.Tensor) or w.dtype != torch.float32 or w.ndim != 2 or not w.numel() or w.stride(1) != 1:
+        raise ValueError("expected a nonempty FP32 [N, K] tensor with unit stride along the last dimension")
+    if group not in GROUPS or w.shape[1] % 32:
+        raise ValueError("group must be 32, 64 or 128 and K a multiple of 32")
+    if scale_dtype not in _DTYPE:
+        raise ValueError("scale_dtype must be bfloat16 or float16")
+    lib = _lib.load()
+    dev = _device_for(w)
+    on_host = w.device.type == "cpu"
+    with _device_guard(dev):
+        wd = w.to(dev, non_blocking=True) if on_host else w
+        n, k = wd.shape
+        g = (k + group - 1) // group
+        codes, scales = _empty(n, k // 2, torch.uint8, dev), _empty(n, g, scale_dtype, dev)
+        z = _empty(n, g, torch.uint8, dev) if zeros else None
+        rc = lib.bfp8_quant_group_w4_f32(wd.data_ptr(), n, k, wd.stride(0) if n > 1 else k, group, codes.data_ptr(),
+                                         scales.data_ptr(), None if z is None else z.data_ptr(), _DTYPE[scale_dtype],
+                                         _stream_ptr(dev))
+        _lib.check(rc, "bfp8_quant_group_w4_f32")
+    if on_host:
+        codes, scales, z = codes.cpu(), scales.cpu(), None if z is None else z.cpu()
+    return codes, scales, z
+
+
+def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, out_dtype=None, check=False, status=None,
+                  wait_limit_cycles=0):
+    """[M, N] = x . W^T (+ bias), W[n, k] = (q[n, k] - z[n, k // group]) * scales[n, k // group].
+
+    x      bf16 or fp16 [M, K], K a multiple of 32; any M, made for up to 32 rows (the weight is read once per 32)
+    codes  uint8 [N, K / 2], q of even k in the low four bits;  scales of x's type [N, ceil(K / group)]
+    zeros  uint8 of scales' shape, 0 .. 15, or None: 8;  bias fp32 [N] or None;  group 32, 64 or 128
+    out    of x's type, or float32 with out_dtype=torch.float32
+    check  read the status word after the launch (one synchronisation) and raise if a bounded wait expired; status as in
+           gemm_block_fp8.  The kernel waits for nothing but its own copies, so calls are unchecked by default.
+    """
+    if (not isinstance(x, torch.Tensor) or x.dtype not in _DTYPE or x.ndim != 2 or x.device.type != "cuda"
+            or (x.shape[1] > 1 and x.stride(1) != 1)):
+        raise ValueError("x must be a bf16 or fp16 [M, K] CUDA tensor with unit column stride")
+    m, k = x.shape
+    dev = x.device
+    if group not in GROUPS or k < 32 or k % 32:
+        raise ValueError("group must be 32, 64 or 128 and K a multiple of 32")
+    if (not isinstance(codes, torch.Tensor) or codes.dtype != torch.uint8 or codes.ndim != 2 or codes.shape[1] * 2 != k
+            or codes.shape[0] < 1 or not codes.is_contiguous() or codes.device != dev):
+        raise ValueError("codes must be contiguous uint8 [N, K / 2] on x's device")
+    n = codes.shape[0]
+    shape = (n, (k + group - 1) // group)
+    if (not isinstance(scales, torch.Tensor) or scales.dtype != x.dtype or scales.shape != shape
+            or not scales.is_contiguous() or scales.device != dev):
+        raise ValueError("scales must be contiguous [N, ceil(K / group)] of x's type on x's device")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != shape or not zeros.is_contiguous()
+                              or zeros.device != dev):
+        raise ValueError("zeros must be contiguous uint8 of the scales' shape on x's device")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()
+                             or bias.device != dev):
+        raise ValueError("bias must be contiguous FP32 [N] on x's device")
+    if out_dtype is None:
+        out_dtype = x.dtype if out is None else out.dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise ValueError("out_dtype must be x's type or float32")
+    if out is not None and (out.dtype != out_dtype or out.shape != (m, n) or (n > 1 and out.stride(1) != 1)
+                            or (m > 1 and out.stride(0) < n) or out.device != dev):
+        raise ValueError("out must be [M, N] of out_dtype on x's device with unit column stride and rows apart")
+    lib = _lib.load()
+    with _device_guard(dev):
+        if out is None:
+            out = _empty(m, n, out_dtype, dev)
+        if m == 0:
+            return out
+        if x.data_ptr() % 16 or (m > 1 and x.stride(0) % 8):
+            x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries
+        st = status if status is not None else _status_buffer(dev) if check else _unread_status_buffer(dev)
+        rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, _DTYPE[x.dtype], codes.data_ptr(),
+                                    scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
+                                    None if bias is None else bias.data_ptr(), out.data_ptr(),
+                                    int(out_dtype == torch.float32), out.stride(0) if m > 1 else n, m, n, k,
+                                    st.data_ptr() + 8, _stream_ptr(dev), wait_limit_cycles)
+        _lib.check(rc, "bfp8_gemm_group_w4")
+        if check and _read_status(st)[1] & _lib.STATUS_WAIT_TIMEOUT:
+            raise _lib.Bfp8Error(_WAIT_TIMEOUT_MSG)
+    return out

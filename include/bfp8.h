@@ -199,7 +199,7 @@ int bfp8_gemm_token_channel(const uint8_t* a_codes, int64_t lda, const float* a_
 int bfp8_gemm_k_split(int64_t m, int64_t n, int64_t k, int token_channel, int sms);
 
 /* Declares, for the whole process, whether the weight operands (w_codes) of the decode-bucket GEMMs (m <= 128:
- * bfp8_gemm_block128, _ex, _swiglu, _push, _noalloc) are at rest.  These kernels are launched so that their
+ * bfp8_gemm_block128, _ex, _swiglu, _push, _noalloc) and of bfp8_gemm_group_w4 are at rest.  These kernels are launched so that their
  * set-up overlaps the end of the previous kernel of the stream, and normally touch no global memory until that
  * kernel has finished.  With on != 0 the caller promises that no work still in flight when such a GEMM is
  * enqueued writes its w_codes (weights were prepared at load time and the device was synchronised since); the
@@ -375,6 +375,29 @@ int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* rout
                             const uint8_t* w_gate_up, const float* s_gate_up, const uint8_t* w_down, const float* s_down,
                             uint16_t* out, int64_t ldo, int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t inter,
                             int native_half, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
+
+/* Product of a few activation rows with a 4-bit weight that has a scale (and a zero point) per group of k:
+ *   out[i, j] = sum_k x[i, k] * (q[j, k] - z[j, k / group]) * s[j, k / group] (+ bias[j])
+ *   x       bf16 (x_dtype BFP8_W4_BF16) or fp16 (BFP8_W4_F16) [m, k], row stride ldx (ldx % 8 == 0, 16-byte aligned)
+ *   codes   uint8 [n, k / 2], contiguous, 16-byte aligned: q of even k in the low, of odd k in the high four bits
+ *   scales  of x's type [n, ceil(k / group)], contiguous;  zeros uint8, the same shape, 0 .. 15, or NULL: 8
+ *   bias    fp32 [n] or NULL;  out of x's type, or fp32 with out_f32 != 0, [m, n], row stride ldo
+ * group 32, 64 or 128, k a multiple of 32 (BFP8_ERR_UNSUPPORTED otherwise; the last group may be short).  q - z is exact,
+ * sums are formed in fp32 in a fixed order, and a group's sum is multiplied by its scale in fp32.  Made for m up to 32 or
+ * so: the weight is read once per 32 rows.  No workspace.  With bfp8_set_weights_at_rest the codes are requested before
+ * the previous kernel of the stream has ended.  status |= WAIT_TIMEOUT if an internal wait gave up.  The reference has no
+ * counterpart. */
+#define BFP8_W4_BF16 0
+#define BFP8_W4_F16  1
+int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const uint8_t* codes, const uint16_t* scales,
+                       const uint8_t* zeros, int group, const float* bias, void* out, int out_f32, int64_t ldo,
+                       int64_t m, int64_t n, int64_t k, uint32_t* status_dev, void* stream, int64_t wait_limit_cycles);
+
+/* fp32 weight [n, k] (row stride ldw) -> the codes, scales and zero points above.  zeros != NULL:
+ * s = round16((max(w, 0) - min(w, 0)) / 15), z = clamp(rne(-min / s), 0, 15); zeros == NULL: s = round16(max|w| / 7),
+ * z = 8.  q = clamp(rne(w / s) + z, 0, 15); a group of zeros, or one whose s rounds to zero, gets s = 1. */
+int bfp8_quant_group_w4_f32(const float* w, int64_t n, int64_t k, int64_t ldw, int group, uint8_t* codes,
+                            uint16_t* scales, uint8_t* zeros, int scale_dtype, void* stream);
 
 #ifdef __cplusplus
 }
