@@ -32,7 +32,7 @@ constexpr long long kDefaultWaitLimit = 2000000000LL;      // about a second
 constexpr int kStageK = 256;                               // k per stage: 128 bytes of a code row
 constexpr int kMaxRows = 256;                              // weight rows per CTA, the largest TMA box
 constexpr int kMaxStages = 16;
-constexpr int kRingBytes = 208 * 1024;
+constexpr int kSmemBytes = 224 * 1024;
 constexpr int kMaxCluster = 8;
 
 struct W4Params {
@@ -48,6 +48,7 @@ struct W4Params {
                                // the phase it waits for cannot be mistaken for an older one of the same parity
   int cluster;
   int out_f32;
+  int scale_vec;               // the scales and zero points of a step can be loaded together
   int w_early;
   long long wait_limit;
   uint32_t* status;
@@ -74,6 +75,11 @@ struct Half16<true> {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
+  // the same from zero
+  static __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+  }
 };
 template <>
 struct Half16<false> {
@@ -91,6 +97,10 @@ struct Half16<false> {
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
   }
 };
 
@@ -118,27 +128,75 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 
 // kNT: activation rows / 8; kMT: 16-row weight tiles per warp (x is read from shared memory once for all of them);
 // kShift: group = 32 << kShift.
-// Warps that multiply; with the producer the sums of 32 rows x 64 weight rows fit in the registers of eight warps.
-__host__ __device__ constexpr int consumers(int nt) { return nt >= 4 ? 7 : 15; }
+constexpr int kMT = 2;                                     // 16-row weight tiles per warp: x is read and permuted once for both
+// Warps that multiply, beside the one that copies: as many as the registers of their sums allow
+__host__ __device__ constexpr int consumers(int nt) { return nt == 1 ? 23 : 15; }
+constexpr int kWarpRows = 16 * kMT;                        // a lane fetches the scales of one row
 
-template <bool kBf16, int kNT, int kMT, int kShift>
+__host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * 128 + mp * kStageK * 2; }
+// {scale, offset} of a warp's rows in the step it works on
+__host__ __device__ constexpr int scale_area(int nt, int groups) { return consumers(nt) * kWarpRows * groups * 8; }
+__host__ __device__ constexpr int ring_bytes(int nt, int groups) { return (kSmemBytes - scale_area(nt, groups)) & ~1023; }
+
+// The scales and zero points of one row in one step as they lie in memory: loaded a step before they are used, so that
+// nothing waits for them
+template <int kGroups>
+struct RawScales {
+  uint32_t s[kGroups / 2];
+  uint32_t z[(kGroups + 3) / 4];
+  __device__ __forceinline__ void load(const W4Params& p, int row, int g0) {
+#pragma unroll
+    for (int i = 0; i < kGroups / 2; ++i) s[i] = 0u;
+#pragma unroll
+    for (int i = 0; i < (kGroups + 3) / 4; ++i) z[i] = 0x08080808u;
+    if (row >= p.n) return;
+    const int64_t at = static_cast<int64_t>(row) * p.groups + g0;
+    if (p.scale_vec) {                                             // groups % kGroups == 0, so a step's groups exist together
+      if (kGroups == 2) {
+        s[0] = __ldg(reinterpret_cast<const uint32_t*>(p.scales + at));
+        if (p.zeros != nullptr) z[0] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + at));
+      } else if (kGroups == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p.scales + at));
+        s[0] = v.x; s[kGroups > 2 ? 1 : 0] = v.y;
+        if (p.zeros != nullptr) z[0] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
+      } else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.scales + at));
+        s[0] = v.x; s[kGroups > 2 ? 1 : 0] = v.y; s[kGroups > 4 ? 2 : 0] = v.z; s[kGroups > 4 ? 3 : 0] = v.w;
+        if (p.zeros != nullptr) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.zeros + at));
+          z[0] = u.x; z[kGroups > 4 ? 1 : 0] = u.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+        if (g0 + j < p.groups) {
+          s[j >> 1] |= static_cast<uint32_t>(__ldg(p.scales + at + j)) << (16 * (j & 1));
+          if (p.zeros != nullptr)
+            z[j >> 2] = (z[j >> 2] & ~(0xffu << (8 * (j & 3)))) | static_cast<uint32_t>(__ldg(p.zeros + at + j)) << (8 * (j & 3));
+        }
+    }
+  }
+};
+
+// kNT: activation rows / 8; kShift: group = 32 << kShift.
+template <bool kBf16, int kNT, int kShift>
 __global__ void __launch_bounds__((consumers(kNT) + 1) * 32, 1)
 w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Params p) {
   using H = Half16<kBf16>;
-  constexpr int kConsumers = consumers(kNT), kThreads = (kConsumers + 1) * 32;
+  constexpr int kConsumers = consumers(kNT), kProducer = kConsumers, kThreads = (kConsumers + 1) * 32;
   constexpr int kMp = kNT * 8;
   constexpr int kXBytes = kMp * kStageK * 2;
   constexpr int kStageGroups = kStageK >> (5 + kShift);            // scale groups per stage: 8, 4, 2
-  constexpr int kHeld = kStageGroups / 2;                          // registers of scales per 16-row tile and stage
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + kRingBytes);
+  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + ring_bytes(kNT, kStageGroups) + scale_area(kNT, kStageGroups));
   volatile uint32_t* abort_flag = &tail->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = p.rows / (16 * kMT);                           // warps across R
+  const int units = p.rows / kWarpRows;                            // warps across R
   const int slices = p.slices;
-  const uint32_t stage_bytes = static_cast<uint32_t>(p.rows) * 128u + kXBytes;
+  const uint32_t stage_bytes = static_cast<uint32_t>(stage_size(p.rows, kMp));
   const int rank = p.cluster > 1 ? static_cast<int>(blockIdx.x) % p.cluster : 0;
   const int n0 = static_cast<int>(blockIdx.x) / p.cluster * p.rows;
   const int m0 = blockIdx.y * kMp;
@@ -166,7 +224,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
       for (int c = 0; c < 4; ++c) acc[a][b][c] = 0.0f;
   const int unit = warp % units, slice = warp / units;
 
-  if (warp == kConsumers) {
+  if (warp == kProducer) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       ptx::prefetch_tensormap(&tmap_w);
@@ -198,38 +256,30 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     }
   } else if (slice < slices) {
     // ------------------------------------------------------------------ consumers
-    ptx::griddep_wait();
     const int g = lane >> 2, t = lane & 3;
     // activation row of column g of the B operand: neighbouring columns lie in different halves of the swizzled 128 bytes
     const int xrow = (g >> 1) + 4 * (g & 1);
-    // scale and zero point of (row lane & 15 of tile a, group 2 r + lane / 16 of step s) in one register
-    uint32_t held[kMT][kHeld];
-    auto fetch = [&](int s) {
-#pragma unroll
-      for (int a = 0; a < kMT; ++a)
-#pragma unroll
-        for (int r = 0; r < kHeld; ++r) {
-          const int row = n0 + (unit * kMT + a) * 16 + (lane & 15), gr = s * kStageGroups + 2 * r + (lane >> 4);
-          uint32_t v = 0u;
-          if (row < p.n && gr < p.groups) {
-            const int64_t at = static_cast<int64_t>(row) * p.groups + gr;
-            v = __ldg(p.scales + at) | ((p.zeros != nullptr ? static_cast<uint32_t>(__ldg(p.zeros + at)) : 8u) << 16);
-          }
-          held[a][r] = v;
-        }
-    };
-    if (step0 + slice < step1) fetch(step0 + slice);
+    const uint32_t area = smem_base + ring_bytes(kNT, kStageGroups) + warp * (kWarpRows * kStageGroups * 8);
+    const uint32_t sbase = area + g * 8;
+    const int row = n0 + unit * kWarpRows + lane;
+    ptx::griddep_wait();
+    RawScales<kStageGroups> raw;
+    if (step0 + slice < step1) raw.load(p, row, (step0 + slice) * kStageGroups);
     int stage = slice, parity = 0;
     for (int s = step0 + slice; s < step1; s += slices) {
+      __syncwarp();                                                // the last step's scales have been read
+#pragma unroll
+      for (int j = 0; j < kStageGroups; ++j) {
+        const uint32_t sc = (raw.s[j >> 1] >> (16 * (j & 1))) & 0xffffu, z = (raw.z[j >> 2] >> (8 * (j & 3))) & 0xffu;
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(area + (j * kWarpRows + lane) * 8), "f"(H::value(sc)),
+                     "r"(H::kMinus + z * 0x10001u) : "memory");
+      }
+      __syncwarp();
+      if (s + slices < step1) raw.load(p, row, (s + slices) * kStageGroups);
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit))) break;
-      const uint32_t wbase = smem_base + stage * stage_bytes + unit * kMT * 2048 + g * 128 + t * 4;
-      const uint32_t xbase = smem_base + stage * stage_bytes + p.rows * 128 + xrow * 128;
-      uint32_t now[kMT][kHeld];
-#pragma unroll
-      for (int a = 0; a < kMT; ++a)
-#pragma unroll
-        for (int r = 0; r < kHeld; ++r) now[a][r] = held[a][r];
-      if (s + slices < step1) fetch(s + slices);
+      // the 128-byte swizzle: chunk c of 16 bytes of row r lies at c ^ (r & 7)
+      const uint32_t wbase = smem_base + stage * stage_bytes + unit * kMT * 2048 + g * 128 + (g << 4) + t * 4;
+      const uint32_t xbase = smem_base + stage * stage_bytes + p.rows * 128 + xrow * 128 + ((t ^ xrow) << 4);
       float part[kMT][kNT][4];
       uint32_t sub0[kMT][2], sub1[kMT][2];
       float scale[kMT][2];
@@ -237,28 +287,19 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
       for (int q = 0; q < kStageK / 32; ++q) {
         constexpr int kMask = (1 << kShift) - 1;
         if ((q & kMask) == 0) {                                    // a new group
-          const int gr = q >> kShift;
 #pragma unroll
-          for (int a = 0; a < kMT; ++a) {
+          for (int a = 0; a < kMT; ++a)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const uint32_t v = __shfl_sync(0xffffffffu, now[a][gr >> 1], (gr & 1) * 16 + g + 8 * r);
-              scale[a][r] = H::value(v & 0xffffu);
-              sub0[a][r] = H::kMinus + (v >> 16) * 0x10001u;       // -(128 + z), fp16 -(1024 + z), in both halves
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=f"(scale[a][r]), "=r"(sub0[a][r])
+                           : "r"(sbase + ((q >> kShift) * kWarpRows + a * 16 + r * 8) * 8));
               if (!kBf16) sub1[a][r] = H::fma(sub0[a][r], H::kOne, H::kStep);      // -(64 + z)
             }
-#pragma unroll
-            for (int b = 0; b < kNT; ++b)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) part[a][b][c] = 0.0f;
-          }
         }
         uint32_t x[kNT][4];
 #pragma unroll
         for (int b = 0; b < kNT; ++b) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (m0 + b * 8 + xrow < p.m)
-            v = lds128(xbase + (q >> 1) * (kMp * 128) + b * 1024 + ((((q & 1) * 4 + t) ^ xrow) << 4));
+          const uint4 v = lds128((xbase ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128) + b * 1024);
           x[b][0] = __byte_perm(v.x, v.z, 0x5410);                 // (k, k + 4) for k = 0 .. 3
           x[b][1] = __byte_perm(v.x, v.z, 0x7632);
           x[b][2] = __byte_perm(v.y, v.w, 0x5410);
@@ -269,7 +310,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
           uint32_t w[2][4];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint32_t lo = lds32(wbase + a * 2048 + r * 1024 + ((q ^ g) << 4)), hi = lo >> 8;
+            const uint32_t lo = lds32((wbase ^ (q << 4)) + a * 2048 + r * 1024), hi = lo >> 8;
             w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
             w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
             if (kBf16) {                                           // seven bits of fraction: no room for a value shifted by four
@@ -282,7 +323,8 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
           }
 #pragma unroll
           for (int b = 0; b < kNT; ++b) {
-            H::mma(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1]);
+            if ((q & kMask) == 0) H::mma0(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1]);
+            else H::mma(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1]);
             H::mma(part[a][b], w[0][2], w[1][2], w[0][3], w[1][3], x[b][2], x[b][3]);
           }
           if ((q & kMask) == kMask)
@@ -302,7 +344,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   // ------------------------------------------------------------------ sums of the slices, then of the cluster's CTAs
   __syncthreads();                                                 // every stage has been read: the ring is free
   float* red = reinterpret_cast<float*>(smem);                     // [slice][activation row][weight row]
-  const int width = units * 16 * kMT;
+  const int width = p.rows;
   if (warp < kConsumers && slice < slices) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -326,7 +368,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   }
   auto store = [&](int i, float v) {
     const int m = i / width, n = n0 + i - m * width;
-    if (i - m * width >= p.rows || n >= p.n) return;
+    if (n >= p.n) return;
     if (p.bias != nullptr) v += __ldg(p.bias + n);
     const int64_t at = static_cast<int64_t>(m0 + m) * p.ldo + n;
     if (p.out_f32) static_cast<float*>(p.out)[at] = v;
@@ -353,40 +395,41 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 }
 
 // Rows per CTA and CTAs per cluster: the fewest bytes for the CTA that has most of them.  A cluster's exchange costs about
-// as much time as a CTA needs for 32 KB.  step: the rows that one warp handles.
+// as much time as a CTA needs for 32 KB.
 struct Plan {
   int rows, cluster;
 };
-Plan w4_plan(int64_t n, int64_t k, int step, int warps, int sms) {
-  const int most = step * warps < kMaxRows ? step * warps : kMaxRows;
+Plan w4_plan(int64_t n, int64_t k, int sms) {
   const int64_t steps = (k + kStageK - 1) / kStageK;
-  Plan best = {step, 1};
+  Plan best = {kWarpRows, 1};
   int64_t best_cost = INT64_MAX;
   for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2) {
     if (cluster > steps) break;
-    for (int rows = step; rows <= most; rows += step) {
+    for (int rows = kWarpRows; rows <= kMaxRows; rows += kWarpRows) {
       const int64_t tiles = (n + rows - 1) / rows, waves = (tiles * cluster + sms - 1) / sms;
-      const int64_t cost = waves * (rows * 128 * ((steps + cluster - 1) / cluster) + 4096) + (cluster > 1 ? 32768 : 0);
+      const int64_t cost = waves * (rows * 128 * ((steps + cluster - 1) / cluster) + 65536 + (cluster > 1 ? 32768 : 0));
       if (cost < best_cost) { best_cost = cost; best = {rows, cluster}; }
     }
   }
   return best;
 }
 
-template <bool kBf16, int kNT, int kMT, int kShift>
+template <bool kBf16, int kNT, int kShift>
 int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  constexpr int smem = 1024 + kRingBytes + static_cast<int>(sizeof(W4Tail));
+  constexpr int kStageGroups = kStageK >> (5 + kShift), kRing = ring_bytes(kNT, kStageGroups);
+  constexpr int smem = 1024 + kRing + scale_area(kNT, kStageGroups) + static_cast<int>(sizeof(W4Tail));
   static_assert(smem <= 227 * 1024, "shared memory of one SM");
-  auto kernel = w4_kernel<kBf16, kNT, kMT, kShift>;
+  auto kernel = w4_kernel<kBf16, kNT, kShift>;
   static DeviceFlags done;
   int rc = ensure_smem_limit(kernel, smem, done);
   if (rc != BFP8_OK) return rc;
-  const Plan plan = w4_plan(p.n, p.k, 16 * kMT, consumers(kNT), sm_count());
+  const Plan plan = w4_plan(p.n, p.k, sm_count());
   p.rows = plan.rows;
   p.cluster = plan.cluster;
-  const int stage_bytes = p.rows * 128 + kNT * 8 * kStageK * 2;
-  const int most = kRingBytes / stage_bytes < kMaxStages ? kRingBytes / stage_bytes : kMaxStages;
-  p.slices = consumers(kNT) / (p.rows / (16 * kMT));
+  const int stage_bytes = stage_size(p.rows, kNT * 8);
+  p.scale_vec = p.groups % kStageGroups == 0 && aligned(p.scales, 2 * kStageGroups) && (p.zeros == nullptr || aligned(p.zeros, kStageGroups));
+  const int most = kRing / stage_bytes < kMaxStages ? kRing / stage_bytes : kMaxStages;
+  p.slices = consumers(kNT) / (p.rows / kWarpRows);
   if (p.slices > most) p.slices = most;
   p.stages = most / p.slices * p.slices;
   alignas(64) CUtensorMap tmap_w, tmap_x;
@@ -413,18 +456,18 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   return BFP8_OK;
 }
 
-template <bool kBf16, int kNT, int kMT>
+template <bool kBf16, int kNT>
 int launch_group(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  if (group == 32) return launch_w4<kBf16, kNT, kMT, 0>(codes, x, ldx, p, st);
-  if (group == 64) return launch_w4<kBf16, kNT, kMT, 1>(codes, x, ldx, p, st);
-  return launch_w4<kBf16, kNT, kMT, 2>(codes, x, ldx, p, st);
+  if (group == 32) return launch_w4<kBf16, kNT, 0>(codes, x, ldx, p, st);
+  if (group == 64) return launch_w4<kBf16, kNT, 1>(codes, x, ldx, p, st);
+  return launch_w4<kBf16, kNT, 2>(codes, x, ldx, p, st);
 }
 
 template <bool kBf16>
 int launch_rows(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  if (p.m <= 8) return launch_group<kBf16, 1, 1>(group, codes, x, ldx, p, st);
-  if (p.m <= 16) return launch_group<kBf16, 2, 2>(group, codes, x, ldx, p, st);
-  return launch_group<kBf16, 4, 4>(group, codes, x, ldx, p, st);
+  if (p.m <= 8) return launch_group<kBf16, 1>(group, codes, x, ldx, p, st);
+  if (p.m <= 16) return launch_group<kBf16, 2>(group, codes, x, ldx, p, st);
+  return launch_group<kBf16, 4>(group, codes, x, ldx, p, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
