@@ -32,7 +32,7 @@ constexpr long long kDefaultWaitLimit = 2000000000LL;      // about a second
 constexpr int kStageK = 256;                               // k per stage: 128 bytes of a code row
 constexpr int kMaxRows = 256;                              // weight rows per CTA, the largest TMA box
 constexpr int kMaxStages = 16;
-constexpr int kSmemBytes = 224 * 1024;
+constexpr int kSmemBytes = 225 * 1024;
 constexpr int kMaxCluster = 8;
 
 struct W4Params {
@@ -43,9 +43,8 @@ struct W4Params {
   int64_t ldo;
   int m, n, k, groups;
   int rows;                    // R
-  int slices;                  // warps that share a row range: they take the stages in turn
-  int stages;                  // ring depth, a multiple of slices: the stage a warp waits for is one it has emptied itself, so
-                               // the phase it waits for cannot be mistaken for an older one of the same parity
+  int slices;                  // warps that share a row range: 2 take a half of each stage's k each
+  int stages;                  // ring depth
   int cluster;
   int out_f32;
   int scale_vec;               // the scales and zero points of a step can be loaded together
@@ -55,7 +54,7 @@ struct W4Params {
 };
 
 struct W4Tail {
-  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages];
   uint32_t abort_flag;
 };
 
@@ -72,12 +71,12 @@ struct Half16<true> {
   static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits << 16); }
   static __device__ __forceinline__ uint16_t round(float v) { return static_cast<uint16_t>(float_to_bf16_bits(v)); }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
   // the same from zero
   static __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
   }
 };
@@ -95,11 +94,11 @@ struct Half16<false> {
   }
   static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
   }
 };
@@ -110,16 +109,6 @@ __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t mag
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
   return r;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -128,40 +117,39 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 
 // kNT: activation rows / 8; kMT: 16-row weight tiles per warp (x is read from shared memory once for all of them);
 // kShift: group = 32 << kShift.
-constexpr int kMT = 2;                                     // 16-row weight tiles per warp: x is read and permuted once for both
-// Warps that multiply, beside the one that copies: as many as the registers of their sums allow
-__host__ __device__ constexpr int consumers(int nt) { return nt == 1 ? 23 : 15; }
-constexpr int kWarpRows = 16 * kMT;                        // a lane fetches the scales of one row
-
+// Warps that multiply, warps that rearrange x (one per 8 activation rows), and one that copies
+__host__ __device__ constexpr int consumers(int nt) { return 15 - nt; }
+constexpr int kThreads = 16 * 32;
+// 16-row weight tiles per warp: with many activation rows two, so that x is read from shared memory once for both
+__host__ __device__ constexpr int tiles(int nt) { return nt >= 4 ? 2 : 1; }
+// Scales are fetched for several steps at once: from the [n, groups] layout one step's scales of a row are 4 to 16 bytes of a
+// 128-byte line, and a warp-wide load costs a cycle per line
+__host__ __device__ constexpr int super_steps(int nt, int shift) { return (shift == 0 ? 2 : 4) / tiles(nt); }
+__host__ __device__ constexpr int step_groups(int shift) { return kStageK >> (5 + shift); }
+__host__ __device__ constexpr int warp_area(int nt, int shift) { return 16 * tiles(nt) * super_steps(nt, shift) * step_groups(shift) * 8; }
+__host__ __device__ constexpr int ring_bytes(int nt, int shift) { return (kSmemBytes - consumers(nt) * warp_area(nt, shift)) & ~1023; }
 __host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * 128 + mp * kStageK * 2; }
-// {scale, offset} of a warp's rows in the step it works on
-__host__ __device__ constexpr int scale_area(int nt, int groups) { return consumers(nt) * kWarpRows * groups * 8; }
-__host__ __device__ constexpr int ring_bytes(int nt, int groups) { return (kSmemBytes - scale_area(nt, groups)) & ~1023; }
 
-// The scales and zero points of one row in one step as they lie in memory: loaded a step before they are used, so that
-// nothing waits for them
+// Scales and zero points of kGroups neighbouring groups of one row as they lie in memory, loaded well before they are used
 template <int kGroups>
 struct RawScales {
   uint32_t s[kGroups / 2];
-  uint32_t z[(kGroups + 3) / 4];
+  uint32_t z[kGroups / 4];
   __device__ __forceinline__ void load(const W4Params& p, int row, int g0) {
 #pragma unroll
     for (int i = 0; i < kGroups / 2; ++i) s[i] = 0u;
 #pragma unroll
-    for (int i = 0; i < (kGroups + 3) / 4; ++i) z[i] = 0x08080808u;
-    if (row >= p.n) return;
+    for (int i = 0; i < kGroups / 4; ++i) z[i] = 0x08080808u;
+    if (row >= p.n || g0 >= p.groups) return;
     const int64_t at = static_cast<int64_t>(row) * p.groups + g0;
-    if (p.scale_vec) {                                             // groups % kGroups == 0, so a step's groups exist together
-      if (kGroups == 2) {
-        s[0] = __ldg(reinterpret_cast<const uint32_t*>(p.scales + at));
-        if (p.zeros != nullptr) z[0] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + at));
-      } else if (kGroups == 4) {
+    if (p.scale_vec) {                                             // groups % kGroups == 0: they exist together
+      if (kGroups == 4) {
         const uint2 v = __ldg(reinterpret_cast<const uint2*>(p.scales + at));
-        s[0] = v.x; s[kGroups > 2 ? 1 : 0] = v.y;
+        s[0] = v.x; s[1] = v.y;
         if (p.zeros != nullptr) z[0] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
       } else {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.scales + at));
-        s[0] = v.x; s[kGroups > 2 ? 1 : 0] = v.y; s[kGroups > 4 ? 2 : 0] = v.z; s[kGroups > 4 ? 3 : 0] = v.w;
+        s[0] = v.x; s[1] = v.y; s[kGroups > 4 ? 2 : 0] = v.z; s[kGroups > 4 ? 3 : 0] = v.w;
         if (p.zeros != nullptr) {
           const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.zeros + at));
           z[0] = u.x; z[kGroups > 4 ? 1 : 0] = u.y;
@@ -181,33 +169,36 @@ struct RawScales {
 
 // kNT: activation rows / 8; kShift: group = 32 << kShift.
 template <bool kBf16, int kNT, int kShift>
-__global__ void __launch_bounds__((consumers(kNT) + 1) * 32, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Params p) {
   using H = Half16<kBf16>;
-  constexpr int kConsumers = consumers(kNT), kProducer = kConsumers, kThreads = (kConsumers + 1) * 32;
+  constexpr int kConsumers = consumers(kNT), kProducer = 15, kMT = tiles(kNT), kWarpRows = 16 * kMT;
   constexpr int kMp = kNT * 8;
   constexpr int kXBytes = kMp * kStageK * 2;
-  constexpr int kStageGroups = kStageK >> (5 + kShift);            // scale groups per stage: 8, 4, 2
+  constexpr int kStepGroups = step_groups(kShift), kSuper = super_steps(kNT, kShift);
+  constexpr int kLaneGroups = kSuper * kStepGroups * kMT / 2;      // 4 or 8: two lanes per row with one tile, one with two
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + ring_bytes(kNT, kStageGroups) + scale_area(kNT, kStageGroups));
+  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + ring_bytes(kNT, kShift) + kConsumers * warp_area(kNT, kShift));
   volatile uint32_t* abort_flag = &tail->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.rows / kWarpRows;                            // warps across R
-  const int slices = p.slices;
+  const int slices = p.slices;                                     // warps across the k of a stage: 1 or 2
   const uint32_t stage_bytes = static_cast<uint32_t>(stage_size(p.rows, kMp));
   const int rank = p.cluster > 1 ? static_cast<int>(blockIdx.x) % p.cluster : 0;
   const int n0 = static_cast<int>(blockIdx.x) / p.cluster * p.rows;
   const int m0 = blockIdx.y * kMp;
   const int all_steps = (p.k + kStageK - 1) / kStageK;
-  const int step0 = static_cast<int>(static_cast<long long>(all_steps) * rank / p.cluster);
-  const int step1 = static_cast<int>(static_cast<long long>(all_steps) * (rank + 1) / p.cluster);
+  // K is cut between pairs of steps, so that a CTA's scales start on the alignment of their loads
+  const int step0 = static_cast<int>(static_cast<long long>((all_steps + 1) / 2) * rank / p.cluster) * 2;
+  const int step1 = min(static_cast<int>(static_cast<long long>((all_steps + 1) / 2) * (rank + 1) / p.cluster) * 2, all_steps);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       ptx::mbar_init(ptx::smem_u32(&tail->full[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), static_cast<uint32_t>(units));
+      ptx::mbar_init(ptx::smem_u32(&tail->ready[s]), kNT);
+      ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), static_cast<uint32_t>(units * slices));
     }
     tail->abort_flag = 0;
     ptx::fence_mbar_init();
@@ -223,6 +214,13 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[a][b][c] = 0.0f;
   const int unit = warp % units, slice = warp / units;
+  const int g = lane >> 2, t = lane & 3;
+  // activation row of column g of the B operand: neighbouring columns lie in different halves of the swizzled 128 bytes
+  const int xrow = (g >> 1) + 4 * (g & 1);
+  uint32_t stage = 0, parity = 0;
+  auto advance = [&] {
+    if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; parity ^= 1u; }
+  };
 
   if (warp == kProducer) {
     // ------------------------------------------------------------------ TMA producer
@@ -238,7 +236,6 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
           ptx::tma_load_2d_hint(smem_base + early * stage_bytes, &tmap_w, full, (step0 + early) * 128, n0, once);
         }
       ptx::griddep_wait();
-      uint32_t stage = 0, parity = 0;
       for (int s = step0; s < step1; ++s) {
         const uint32_t full = ptx::smem_u32(&tail->full[stage]), dst = smem_base + stage * stage_bytes;
         if (early > 0) {
@@ -251,93 +248,114 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 #pragma unroll
         for (int b = 0; b < kStageK / 64; ++b)
           ptx::tma_load_2d(dst + p.rows * 128 + b * kMp * 128, &tmap_x, full, s * kStageK + b * 64, m0);
-        if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; parity ^= 1u; }
+        advance();
       }
+    }
+  } else if (warp >= kConsumers) {
+    // ------------------------------------------------------------------ x of 8 rows: pairs (k, k + 4) side by side, once for all consumers
+    const uint32_t first = p.rows * 128 + ((warp - kConsumers) * 8 + xrow) * 128 + ((t ^ xrow) << 4);
+    for (int s = step0; s < step1; ++s) {
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit))) break;
+      uint8_t* at = smem + stage * stage_bytes;
+      uint4 v[kStageK / 32];
+#pragma unroll
+      for (int q = 0; q < kStageK / 32; ++q) v[q] = *reinterpret_cast<const uint4*>(at + (first ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128));
+#pragma unroll
+      for (int q = 0; q < kStageK / 32; ++q)
+        *reinterpret_cast<uint4*>(at + (first ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128)) =
+            make_uint4(__byte_perm(v[q].x, v[q].z, 0x5410), __byte_perm(v[q].x, v[q].z, 0x7632),
+                       __byte_perm(v[q].y, v[q].w, 0x5410), __byte_perm(v[q].y, v[q].w, 0x7632));
+      __syncwarp();
+      ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->ready[stage]), lane);
+      advance();
     }
   } else if (slice < slices) {
     // ------------------------------------------------------------------ consumers
-    const int g = lane >> 2, t = lane & 3;
-    // activation row of column g of the B operand: neighbouring columns lie in different halves of the swizzled 128 bytes
-    const int xrow = (g >> 1) + 4 * (g & 1);
-    const uint32_t area = smem_base + ring_bytes(kNT, kStageGroups) + warp * (kWarpRows * kStageGroups * 8);
-    const uint32_t sbase = area + g * 8;
-    const int row = n0 + unit * kWarpRows + lane;
+    const uint32_t area = ring_bytes(kNT, kShift) + warp * warp_area(kNT, kShift);
+    // this lane's share of the scales: a row, and with one tile per warp one half of the groups
+    const int row = kMT == 1 ? lane & 15 : lane, share = kMT == 1 ? (lane >> 4) * kLaneGroups : 0;
+    const uint32_t w_first = unit * kMT * 2048 + g * 128 + (g << 4) + t * 4;      // chunk c of 16 bytes of row r lies at c ^ (r & 7)
+    const uint32_t x_first = p.rows * 128 + xrow * 128 + ((t ^ xrow) << 4);
     ptx::griddep_wait();
-    RawScales<kStageGroups> raw;
-    if (step0 + slice < step1) raw.load(p, row, (step0 + slice) * kStageGroups);
-    int stage = slice, parity = 0;
-    for (int s = step0 + slice; s < step1; s += slices) {
-      __syncwarp();                                                // the last step's scales have been read
+    RawScales<kLaneGroups> raw;
+    raw.load(p, n0 + unit * kWarpRows + row, step0 * kStepGroups + share);
+    for (int s0 = step0; s0 < step1; s0 += kSuper) {
+      __syncwarp();                                                // the last scales have been read
 #pragma unroll
-      for (int j = 0; j < kStageGroups; ++j) {
+      for (int j = 0; j < kLaneGroups; ++j) {
         const uint32_t sc = (raw.s[j >> 1] >> (16 * (j & 1))) & 0xffffu, z = (raw.z[j >> 2] >> (8 * (j & 3))) & 0xffu;
-        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(area + (j * kWarpRows + lane) * 8), "f"(H::value(sc)),
-                     "r"(H::kMinus + z * 0x10001u) : "memory");
+        *reinterpret_cast<uint2*>(smem + area + ((share + j) * kWarpRows + row) * 8) =
+            make_uint2(__float_as_uint(H::value(sc)), H::kMinus + z * 0x10001u);
       }
       __syncwarp();
-      if (s + slices < step1) raw.load(p, row, (s + slices) * kStageGroups);
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit))) break;
-      // the 128-byte swizzle: chunk c of 16 bytes of row r lies at c ^ (r & 7)
-      const uint32_t wbase = smem_base + stage * stage_bytes + unit * kMT * 2048 + g * 128 + (g << 4) + t * 4;
-      const uint32_t xbase = smem_base + stage * stage_bytes + p.rows * 128 + xrow * 128 + ((t ^ xrow) << 4);
-      float part[kMT][kNT][4];
-      uint32_t sub0[kMT][2], sub1[kMT][2];
-      float scale[kMT][2];
+      if (s0 + kSuper < step1) raw.load(p, n0 + unit * kWarpRows + row, (s0 + kSuper) * kStepGroups + share);
+      const int s1 = min(s0 + kSuper, step1);
+      bool ok = true;
+      for (int s = s0; s < s1; ++s) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit) &&
+                                         ptx::mbar_wait(ptx::smem_u32(&tail->ready[stage]), parity, abort_flag, p.wait_limit));
+        if (!ok) break;
+        const uint8_t* at = smem + stage * stage_bytes;
+        const uint8_t* scales = smem + area + ((s - s0) * kStepGroups * kWarpRows + g) * 8;
+#pragma unroll 1
+        for (int half = slice; half < 2; half += slices) {         // 128 k
+          float part[kMT][kNT][4];
+          uint32_t sub0[kMT][2], sub1[kMT][2];
+          float scale[kMT][2];
 #pragma unroll
-      for (int q = 0; q < kStageK / 32; ++q) {
-        constexpr int kMask = (1 << kShift) - 1;
-        if ((q & kMask) == 0) {                                    // a new group
+          for (int q = 0; q < 4; ++q) {
+            constexpr int kMask = (1 << kShift) - 1;
+            if ((q & kMask) == 0) {                                // a new group
 #pragma unroll
-          for (int a = 0; a < kMT; ++a)
+              for (int a = 0; a < kMT; ++a)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=f"(scale[a][r]), "=r"(sub0[a][r])
-                           : "r"(sbase + ((q >> kShift) * kWarpRows + a * 16 + r * 8) * 8));
-              if (!kBf16) sub1[a][r] = H::fma(sub0[a][r], H::kOne, H::kStep);      // -(64 + z)
+                for (int r = 0; r < 2; ++r) {
+                  const uint2 v = *reinterpret_cast<const uint2*>(scales + (((half * 4 + q) >> kShift) * kWarpRows + a * 16 + r * 8) * 8);
+                  scale[a][r] = __uint_as_float(v.x);
+                  sub0[a][r] = v.y;
+                  if (!kBf16) sub1[a][r] = H::fma(sub0[a][r], H::kOne, H::kStep);      // -(64 + z)
+                }
             }
-        }
-        uint32_t x[kNT][4];
-#pragma unroll
-        for (int b = 0; b < kNT; ++b) {
-          const uint4 v = lds128((xbase ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128) + b * 1024);
-          x[b][0] = __byte_perm(v.x, v.z, 0x5410);                 // (k, k + 4) for k = 0 .. 3
-          x[b][1] = __byte_perm(v.x, v.z, 0x7632);
-          x[b][2] = __byte_perm(v.y, v.w, 0x5410);
-          x[b][3] = __byte_perm(v.y, v.w, 0x7632);
-        }
-#pragma unroll
-        for (int a = 0; a < kMT; ++a) {
-          uint32_t w[2][4];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t lo = lds32((wbase ^ (q << 4)) + a * 2048 + r * 1024), hi = lo >> 8;
-            w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-            w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-            if (kBf16) {                                           // seven bits of fraction: no room for a value shifted by four
-              w[r][1] = H::fma(pick(lo >> 4, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-              w[r][3] = H::fma(pick(lo >> 12, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-            } else {                                               // 1024 + 16 q, times 1/16
-              w[r][1] = H::fma(pick(lo, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
-              w[r][3] = H::fma(pick(hi, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
-            }
-          }
-#pragma unroll
-          for (int b = 0; b < kNT; ++b) {
-            if ((q & kMask) == 0) H::mma0(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1]);
-            else H::mma(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1]);
-            H::mma(part[a][b], w[0][2], w[1][2], w[0][3], w[1][3], x[b][2], x[b][3]);
-          }
-          if ((q & kMask) == kMask)
+            uint4 x[kNT];
 #pragma unroll
             for (int b = 0; b < kNT; ++b)
+              x[b] = *reinterpret_cast<const uint4*>(at + (x_first ^ ((q & 1) << 6)) + (half * 2 + (q >> 1)) * (kMp * 128) + b * 1024);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) acc[a][b][c] = fmaf(part[a][b][c], scale[a][c >> 1], acc[a][b][c]);
+            for (int a = 0; a < kMT; ++a) {
+              uint32_t w[2][4];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const uint32_t lo = *reinterpret_cast<const uint32_t*>(at + (w_first ^ (q << 4) ^ (half << 6)) + a * 2048 + r * 1024);
+                const uint32_t hi = lo >> 8;
+                w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+                w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+                if (kBf16) {                                       // seven bits of fraction: no room for a value shifted by four
+                  w[r][1] = H::fma(pick(lo >> 4, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+                  w[r][3] = H::fma(pick(lo >> 12, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
+                } else {                                           // 1024 + 16 q, times 1/16
+                  w[r][1] = H::fma(pick(lo, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
+                  w[r][3] = H::fma(pick(hi, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
+                }
+              }
+#pragma unroll
+              for (int b = 0; b < kNT; ++b) {
+                if ((q & kMask) == 0) H::mma0(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
+                else H::mma(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
+                H::mma(part[a][b], w[0][2], w[1][2], w[0][3], w[1][3], x[b].z, x[b].w);
+              }
+              if ((q & kMask) == kMask)
+#pragma unroll
+                for (int b = 0; b < kNT; ++b)
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) acc[a][b][c] = fmaf(part[a][b][c], scale[a][c >> 1], acc[a][b][c]);
+            }
+          }
         }
+        __syncwarp();
+        ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->empty[stage]), lane);
+        advance();
       }
-      __syncwarp();
-      ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->empty[stage]), lane);
-      stage += slices;
-      if (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
+      if (!ok) break;
     }
   }
 
@@ -346,7 +364,6 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   float* red = reinterpret_cast<float*>(smem);                     // [slice][activation row][weight row]
   const int width = p.rows;
   if (warp < kConsumers && slice < slices) {
-    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int a = 0; a < kMT; ++a)
 #pragma unroll
@@ -394,20 +411,30 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   if (threadIdx.x == 0 && tail->abort_flag != 0) atomicOr(p.status, BFP8_STATUS_WAIT_TIMEOUT);
 }
 
-// Rows per CTA and CTAs per cluster: the fewest bytes for the CTA that has most of them.  A cluster's exchange costs about
-// as much time as a CTA needs for 32 KB.
+// Rows per CTA and CTAs per cluster: the least time for the CTA that has most to do.  Measured on B200, in 0.01 us: a warp
+// gets through 2 KB of codes per us, a CTA through its share of the HBM rate (44 KB per us) at most, a wave of CTAs takes
+// 1.5 us to start and a cluster 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with clusters of four,
+// 7.2 us without; 1 row x 1024 x 1024: 3.0 us without, 4.4 us with pairs).  resident(c): clusters of c CTAs that the device
+// holds at once, fewer than its SMs / c where an SM's neighbours are not whole clusters.
 struct Plan {
   int rows, cluster;
 };
-Plan w4_plan(int64_t n, int64_t k, int sms) {
+template <typename Resident>
+Plan w4_plan(int64_t n, int64_t k, int nt, Resident resident) {
   const int64_t steps = (k + kStageK - 1) / kStageK;
-  Plan best = {kWarpRows, 1};
+  const int step = 16 * tiles(nt), most = step * consumers(nt) < kMaxRows ? step * consumers(nt) : kMaxRows;
+  Plan best = {step, 1};
   int64_t best_cost = INT64_MAX;
   for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2) {
-    if (cluster > steps) break;
-    for (int rows = kWarpRows; rows <= kMaxRows; rows += kWarpRows) {
-      const int64_t tiles = (n + rows - 1) / rows, waves = (tiles * cluster + sms - 1) / sms;
-      const int64_t cost = waves * (rows * 128 * ((steps + cluster - 1) / cluster) + 65536 + (cluster > 1 ? 32768 : 0));
+    if (cluster > (steps + 1) / 2) break;
+    const int64_t together = resident(cluster);
+    if (together <= 0) continue;
+    for (int rows = step; rows <= most; rows += step) {
+      const int64_t waves = ((n + rows - 1) / rows + together - 1) / together;
+      const int units = rows / step, warps = 2 * units <= consumers(nt) ? 2 * units : units;
+      const int64_t rate = warps * 20 < 440 ? warps * 20 : 440;    // 0.1 KB per us
+      const int64_t each = ((steps + 1) / 2 + cluster - 1) / cluster * 2;
+      const int64_t cost = waves * (rows * each * 125 / rate + 150 + (cluster > 1 ? 120 : 0));
       if (cost < best_cost) { best_cost = cost; best = {rows, cluster}; }
     }
   }
@@ -416,41 +443,51 @@ Plan w4_plan(int64_t n, int64_t k, int sms) {
 
 template <bool kBf16, int kNT, int kShift>
 int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  constexpr int kStageGroups = kStageK >> (5 + kShift), kRing = ring_bytes(kNT, kStageGroups);
-  constexpr int smem = 1024 + kRing + scale_area(kNT, kStageGroups) + static_cast<int>(sizeof(W4Tail));
+  constexpr int kRing = ring_bytes(kNT, kShift);
+  constexpr int smem = 1024 + kRing + consumers(kNT) * warp_area(kNT, kShift) + static_cast<int>(sizeof(W4Tail));
+  constexpr int kLaneGroups = super_steps(kNT, kShift) * step_groups(kShift) * tiles(kNT) / 2;
   static_assert(smem <= 227 * 1024, "shared memory of one SM");
+  static_assert(kLaneGroups == 4 || kLaneGroups == 8, "what RawScales loads at once");
+  static_assert(kRing / stage_size(kMaxRows, kNT * 8) >= 2, "two stages at least");
   auto kernel = w4_kernel<kBf16, kNT, kShift>;
   static DeviceFlags done;
   int rc = ensure_smem_limit(kernel, smem, done);
   if (rc != BFP8_OK) return rc;
-  const Plan plan = w4_plan(p.n, p.k, sm_count());
-  p.rows = plan.rows;
-  p.cluster = plan.cluster;
-  const int stage_bytes = stage_size(p.rows, kNT * 8);
-  p.scale_vec = p.groups % kStageGroups == 0 && aligned(p.scales, 2 * kStageGroups) && (p.zeros == nullptr || aligned(p.zeros, kStageGroups));
-  const int most = kRing / stage_bytes < kMaxStages ? kRing / stage_bytes : kMaxStages;
-  p.slices = consumers(kNT) / (p.rows / kWarpRows);
-  if (p.slices > most) p.slices = most;
-  p.stages = most / p.slices * p.slices;
-  alignas(64) CUtensorMap tmap_w, tmap_x;
-  rc = make_tensor_map_2d(&tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, p.k / 2, p.n, p.k / 2, 128, p.rows);
-  if (rc != BFP8_OK) return rc;
-  rc = make_tensor_map_2d(&tmap_x, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, p.k, p.m,
-                          ldx * 2, 64, kNT * 8);
-  if (rc != BFP8_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>((p.m + kNT * 8 - 1) / (kNT * 8)), 1);
-  cfg.blockDim = dim3((consumers(kNT) + 1) * 32, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
+  static ClusterCaps caps;
+  const Plan plan = w4_plan(p.n, p.k, kNT, [&](int cluster) -> int {
+    if (cluster == 1) return sm_count();
+    cudaLaunchConfig_t ask = cfg;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    ask.gridDim = dim3(static_cast<unsigned>(cluster), 1, 1);
+    ask.attrs = attr + 1;
+    ask.numAttrs = 1;
+    return max_active_clusters(kernel, ask, cluster, caps);
+  });
+  p.rows = plan.rows;
+  p.cluster = plan.cluster;
+  p.scale_vec = p.groups % kLaneGroups == 0 && aligned(p.scales, 2 * kLaneGroups) && (p.zeros == nullptr || aligned(p.zeros, kLaneGroups));
+  p.slices = p.rows / (16 * tiles(kNT)) * 2 <= consumers(kNT) ? 2 : 1;
+  const int most = kRing / stage_size(p.rows, kNT * 8);
+  p.stages = most < kMaxStages ? most : kMaxStages;
+  alignas(64) CUtensorMap tmap_w, tmap_x;
+  rc = make_tensor_map_2d(&tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, p.k / 2, p.n, p.k / 2, 128, p.rows);
+  if (rc != BFP8_OK) return rc;
+  rc = make_tensor_map_2d(&tmap_x, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, p.k, p.m,
+                          ldx * 2, 64, kNT * 8);
+  if (rc != BFP8_OK) return rc;
+  cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>((p.m + kNT * 8 - 1) / (kNT * 8)), 1);
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
   BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmap_w, tmap_x, p));
   return BFP8_OK;
