@@ -31,6 +31,7 @@ constexpr int kMaxTokens = 128;
 constexpr int kMaxTopK = 32;
 constexpr int kMaxSlots = 2048;        // tokens * top_k
 constexpr int kMaxExperts = 512;
+constexpr int kMaxWidth = 1 << 16;     // h and inter: a phase's units fit 32 bits
 constexpr int kMaxGrid = 256;          // the workspace holds this many CTAs' partial sums
 constexpr long long kDefaultWaitLimit = 2000000000LL;      // about a second
 
@@ -58,45 +59,46 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 
 // Largest keys first, ties to the lowest index.  Lane j (j < k) returns the j-th choice and its weight.
+template <int kPer>
 __device__ __forceinline__ void topk_token(const float* __restrict__ row, int experts, int k, const RouteRule& r, int lane,
                                            int& my_id, float& my_weight) {
-  constexpr int kPer = kMaxExperts / 32;
-  const int per = (experts + 31) >> 5;
-  float score[kPer];
+  float score[kPer], bias[kPer];
   uint32_t key[kPer];
   float top = -INFINITY;
+  // all loads on their way before the first is used
 #pragma unroll
-  for (int q = 0; q < kPer; ++q) {
-    key[q] = 0u;
-    score[q] = 0.0f;
-    if (q < per) {
-      const int e = q * 32 + lane;
-      if (e < experts) {
-        score[q] = __ldcg(row + e);
-        key[q] = order_key(r.bias != nullptr ? score[q] + __ldg(r.bias + e) : score[q]);
-      }
-    }
-  }
+  for (int q = 0; q < kPer; ++q) score[q] = __ldcg(row + min(q * 32 + lane, experts - 1));
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) bias[q] = r.bias != nullptr ? __ldg(r.bias + min(q * 32 + lane, experts - 1)) : 0.0f;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) key[q] = q * 32 + lane < experts ? order_key(score[q] + bias[q]) : 0u;
   my_id = -1;
   float my_score = 0.0f;
-  for (int j = 0; j < k; ++j) {
-    uint32_t best = 0u;
-    int best_q = 0;
-    float best_score = 0.0f;
+  // every lane keeps the largest of its own keys; only the lane whose key was taken looks for its next one
+  uint32_t best = 0u;
+  int best_q = 0;
+  float best_score = 0.0f;
+  auto own_best = [&] {
+    best = 0u;
 #pragma unroll
     for (int q = 0; q < kPer; ++q)
-      if (q < per && key[q] > best) { best = key[q]; best_q = q; best_score = score[q]; }
+      if (key[q] > best) { best = key[q]; best_q = q; best_score = score[q]; }
+  };
+  own_best();
+  for (int j = 0; j < k; ++j) {
     const uint32_t most = __reduce_max_sync(0xffffffffu, best);
     const uint32_t mine = best == most ? static_cast<uint32_t>(best_q * 32 + lane) : 0xffffffffu;
     const uint32_t id = __reduce_min_sync(0xffffffffu, mine);
     const float s = __shfl_sync(0xffffffffu, best_score, id & 31u);
+    if (j == 0) top = s;
+    if (lane == j) { my_id = static_cast<int>(id); my_score = s; }
     if (mine == id) {
 #pragma unroll
       for (int q = 0; q < kPer; ++q)
         if (q == best_q) key[q] = 0u;
+      own_best();
     }
-    if (j == 0) top = s;
-    if (lane == j) { my_id = static_cast<int>(id); my_score = s; }
+    __syncwarp();
   }
   float w = lane < k ? my_score : 0.0f;
   if (r.softmax) {
@@ -107,7 +109,7 @@ __device__ __forceinline__ void topk_token(const float* __restrict__ row, int ex
       sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < kPer; ++q)
-        if (q < per && q * 32 + lane < experts) sum += expf(score[q] - top);
+        if (q * 32 + lane < experts) sum += expf(score[q] - top);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -121,6 +123,13 @@ __device__ __forceinline__ void topk_token(const float* __restrict__ row, int ex
   my_weight = w * r.scale;
 }
 
+__device__ __forceinline__ void topk_any(const float* __restrict__ row, int experts, int k, const RouteRule& r, int lane, int& my_id,
+                                         float& my_weight) {
+  if (experts <= 128) topk_token<4>(row, experts, k, r, lane, my_id, my_weight);
+  else if (experts <= 256) topk_token<8>(row, experts, k, r, lane, my_id, my_weight);
+  else topk_token<kMaxExperts / 32>(row, experts, k, r, lane, my_id, my_weight);
+}
+
 __global__ void __launch_bounds__(128)
 moe_topk_kernel(const float* __restrict__ scores, int64_t tokens, int experts, int k, RouteRule rule, int32_t* __restrict__ ids,
                 float* __restrict__ weights) {
@@ -131,7 +140,7 @@ moe_topk_kernel(const float* __restrict__ scores, int64_t tokens, int experts, i
   const int lane = threadIdx.x & 31;
   int id;
   float w;
-  topk_token(scores + t * experts, experts, k, rule, lane, id, w);
+  topk_any(scores + t * experts, experts, k, rule, lane, id, w);
   if (lane < k) {
     ids[t * k + lane] = id;
     weights[t * k + lane] = w;
@@ -176,69 +185,91 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int c, int h, bool v
   return v;
 }
 
-// One warp: the scores of kE experts for kT tokens.  A score decides which experts run, so its sum is held more exactly
-// than fp32 would: products of bf16 numbers are exact in fp32, 16 of them are added in fp32 (an error of a few parts in
-// 10^8 of the score's spread) and the sums of 16 in fp64, which B200 adds at half the fp32 rate.
-template <int kT, int kE>
-__device__ __forceinline__ void router_scores(const FrontParams& p, int64_t t0, int e0, int lane) {
-  double acc[kT][kE];
-#pragma unroll
-  for (int a = 0; a < kT; ++a)
-#pragma unroll
-    for (int b = 0; b < kE; ++b) acc[a][b] = 0.0;
+// A score decides which experts run, so its sum is held more exactly than fp32 would: products of bf16 numbers are exact in
+// fp32, 16 or 32 of them are added in fp32 from zero (off by a few parts in 10^8 of the score's spread) and these sums in
+// fp64, which B200 adds at half the fp32 rate.
+__device__ __forceinline__ float score_of(const FrontParams& p, double sum) {
+  const float l = static_cast<float>(sum);
+  return p.sigmoid ? static_cast<float>(1.0 / (1.0 + exp(-static_cast<double>(l)))) : l;
+}
+
+// Few tokens: one warp per token and expert.
+__device__ __forceinline__ void router_dot(const FrontParams& p, int64_t t, int e, int lane) {
+  double acc = 0.0;
   const bool vec = p.vec != 0;
+  const uint16_t *xr = p.x + t * p.ldx, *wr = p.router + e * p.ldr;
   for (int c = lane * 8; c < p.h; c += 512) {
-    float w[kE][16];
+    float s = 0.0f;
 #pragma unroll
-    for (int b = 0; b < kE; ++b)
+    for (int u = 0; u < 2; ++u) {
+      const uint4 w = load8(wr, c + 256 * u, p.h, vec), v = load8(xr, c + 256 * u, p.h, vec);
+      const uint32_t *a = reinterpret_cast<const uint32_t*>(&w), *b = reinterpret_cast<const uint32_t*>(&v);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (e0 + b < p.experts) v = load8(p.router + (e0 + b) * p.ldr, c + 256 * u, p.h, vec);
-        const uint32_t* r = reinterpret_cast<const uint32_t*>(&v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[b][8 * u + 2 * j] = bf16_lo_to_float(r[j]);
-          w[b][8 * u + 2 * j + 1] = bf16_hi_to_float(r[j]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        s = fmaf(bf16_lo_to_float(a[j]), bf16_lo_to_float(b[j]), s);
+        s = fmaf(bf16_hi_to_float(a[j]), bf16_hi_to_float(b[j]), s);
       }
-#pragma unroll
-    for (int a = 0; a < kT; ++a) {
-      if (t0 + a >= p.t) continue;
-      float s[kE];
-#pragma unroll
-      for (int b = 0; b < kE; ++b) s[b] = 0.0f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint4 v = load8(p.x + (t0 + a) * p.ldx, c + 256 * u, p.h, vec);
-        const uint32_t* r = reinterpret_cast<const uint32_t*>(&v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float lo = bf16_lo_to_float(r[j]), hi = bf16_hi_to_float(r[j]);
-#pragma unroll
-          for (int b = 0; b < kE; ++b) {
-            s[b] = fmaf(lo, w[b][8 * u + 2 * j], s[b]);
-            s[b] = fmaf(hi, w[b][8 * u + 2 * j + 1], s[b]);
-          }
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < kE; ++b) acc[a][b] += static_cast<double>(s[b]);
     }
+    acc += static_cast<double>(s);
   }
 #pragma unroll
-  for (int a = 0; a < kT; ++a)
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0) p.scores[t * p.experts + e] = score_of(p, acc);
+}
+
+// More tokens: a block has 16 experts (the M dimension of mma.sync) and 8 kB tokens (N); its warps take turns in K, 32 at a
+// time, each product of 32 starting from zero.  A thread's operand registers are 8 consecutive k of its rows as they lie in
+// memory: which k a register stands for is free as long as both operands agree.  (128 tokens, 256 experts, H = 4096: plain
+// multiplications, each token's row read again for every two experts, took 46 us where this takes 7.)
+template <int kB>
+__device__ __forceinline__ void router_tile(const FrontParams& p, int64_t t0, int e0, double* red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const bool vec = p.vec != 0;
+  double acc[kB][4];
 #pragma unroll
-    for (int b = 0; b < kE; ++b) {
-      double v = acc[a][b];
+  for (int b = 0; b < kB; ++b)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == (a * kE + b) % 32 && t0 + a < p.t && e0 + b < p.experts) {
-        float l = static_cast<float>(v);
-        if (p.sigmoid) l = static_cast<float>(1.0 / (1.0 + exp(-static_cast<double>(l))));
-        p.scores[(t0 + a) * p.experts + e0 + b] = l;
-      }
+    for (int c = 0; c < 4; ++c) acc[b][c] = 0.0;
+  const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+  const uint16_t *r0 = p.router + static_cast<int64_t>(e0 + g) * p.ldr, *r1 = r0 + 8 * p.ldr;
+  const bool has0 = e0 + g < p.experts, has1 = e0 + g + 8 < p.experts;
+#pragma unroll 2
+  for (int c = warp * 32; c < p.h; c += kFrontWarps * 32) {
+    const int k = c + t * 8;
+    const uint4 w0 = has0 ? load8(r0, k, p.h, vec) : none, w1 = has1 ? load8(r1, k, p.h, vec) : none;
+    uint4 x[kB];
+#pragma unroll
+    for (int b = 0; b < kB; ++b) {
+      const int64_t row = t0 + b * 8 + g;
+      x[b] = row < p.t ? load8(p.x + row * p.ldx, k, p.h, vec) : none;
     }
+#pragma unroll
+    for (int b = 0; b < kB; ++b) {
+      float s[4];
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+          : "=f"(s[0]), "=f"(s[1]), "=f"(s[2]), "=f"(s[3])
+          : "r"(w0.x), "r"(w1.x), "r"(w0.y), "r"(w1.y), "r"(x[b].x), "r"(x[b].y), "f"(0.0f));
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(s[0]), "+f"(s[1]), "+f"(s[2]), "+f"(s[3]) : "r"(w0.z), "r"(w1.z), "r"(w0.w), "r"(w1.w), "r"(x[b].z), "r"(x[b].w));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[b][j] += static_cast<double>(s[j]);
+    }
+  }
+  // the warps' sums, [warp][token][expert]
+#pragma unroll
+  for (int b = 0; b < kB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[(warp * 8 * kB + b * 8 + 2 * t + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[b][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 8 * kB * 16; i += kFrontWarps * 32) {
+    const int64_t token = t0 + i / 16;
+    const int e = e0 + i % 16;
+    if (token < p.t && e < p.experts) {
+      double v = 0.0;
+      for (int w = 0; w < kFrontWarps; ++w) v += red[w * 8 * kB * 16 + i];
+      p.scores[token * p.experts + e] = score_of(p, v);
+    }
+  }
 }
 
 // Scale of a group whose largest magnitude has these bits; NaN where that is inf or NaN, so the whole group becomes NaN.
@@ -272,9 +303,11 @@ __device__ __forceinline__ void quantize_group(const FrontParams& p, int64_t t, 
   if (lane == 0) p.scales[static_cast<int64_t>(g) * p.t + t] = p.half ? scale * 2.0f : scale;
 }
 
-template <int kT, int kE>
+// kB: 8-token columns of a router block, 0: one warp per token and expert
+template <int kB>
 __global__ void __launch_bounds__(kFrontWarps * 32)
 moe_front_kernel(const FrontParams p) {
+  __shared__ double red[kB > 0 ? kFrontWarps * 8 * kB * 16 : 1];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -285,25 +318,32 @@ moe_front_kernel(const FrontParams p) {
     if (item < p.t * p.groups) quantize_group(p, item / p.groups, static_cast<int>(item % p.groups), lane);
     return;
   }
-  const int64_t item = static_cast<int64_t>(blockIdx.x - p.quant_blocks) * kFrontWarps + warp;
-  // the warps of a block share their tokens (through L1) and differ in their experts
-  const int eb = (p.experts + kE - 1) / kE;
-  const int64_t t0 = item / eb * kT;
-  if (t0 < p.t) router_scores<kT, kE>(p, t0, static_cast<int>(item % eb) * kE, lane);
+  const int64_t block = blockIdx.x - p.quant_blocks;
+  if (kB == 0) {
+    const int64_t item = block * kFrontWarps + warp;
+    if (item < p.t * p.experts) router_dot(p, item / p.experts, static_cast<int>(item % p.experts), lane);
+  } else {
+    const int eb = (p.experts + 15) / 16;
+    router_tile<kB == 0 ? 1 : kB>(p, block / eb * (8 * kB), static_cast<int>(block % eb) * 16, red);
+  }
 }
 
 int launch_front(FrontParams& p, cudaStream_t st) {
   const int64_t quant = p.quant_blocks ? (p.t * p.groups + kFrontWarps - 1) / kFrontWarps : 0;
   p.quant_blocks = static_cast<int>(quant);
-  const bool few = p.t <= 4;
+  const int columns = p.t <= 4 ? 0 : p.t <= 8 ? 1 : p.t <= 16 ? 2 : 4;
   int64_t route = 0;
-  if (p.router != nullptr) {
-    const int64_t tokens = few ? p.t : (p.t + 7) / 8, experts = few ? p.experts : (p.experts + 1) / 2;
-    route = (tokens * experts + kFrontWarps - 1) / kFrontWarps;
-  }
+  if (p.router != nullptr)
+    route = columns == 0 ? (p.t * p.experts + kFrontWarps - 1) / kFrontWarps
+                         : (p.t + 8 * columns - 1) / (8 * columns) * ((p.experts + 15) / 16);
   if (quant + route > 2147483647LL) return BFP8_ERR_SHAPE;
-  const dim3 grid(static_cast<unsigned>(quant + route));
-  return launch_overlapped(few ? moe_front_kernel<1, 1> : moe_front_kernel<8, 2>, grid, dim3(kFrontWarps * 32), 0, st, p);
+  const dim3 grid(static_cast<unsigned>(quant + route)), block(kFrontWarps * 32);
+  switch (columns) {
+    case 0: return launch_overlapped(moe_front_kernel<0>, grid, block, 0, st, p);
+    case 1: return launch_overlapped(moe_front_kernel<1>, grid, block, 0, st, p);
+    case 2: return launch_overlapped(moe_front_kernel<2>, grid, block, 0, st, p);
+    default: return launch_overlapped(moe_front_kernel<4>, grid, block, 0, st, p);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -332,6 +372,7 @@ struct Routing {
   int16_t slot_expert[kMaxSlots];      // -1: no expert here
   uint16_t count[kMaxExperts];
   uint16_t start[kMaxExperts];
+  uint16_t chunk[kMaxExperts];
 };
 struct Exchange {
   float value[2][8][128];              // [up to the gate side / gate to the up side][column][row]
@@ -342,7 +383,7 @@ struct Tail {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t tmem_full[2][kAccBufs], tmem_empty[2][kAccBufs];
   float scale[kAccBufs][2][64];
-  uint16_t pos_of_slot[kMaxSlots];     // place of a slot in the order of experts, 0xffff: none
+  uint16_t place_of_slot[kMaxSlots];   // chunk * 64 + column of a slot, 0xffff: none
   uint8_t token_of_pos[kMaxSlots];
   uint16_t chunk_expert[kMaxChunks];
   uint16_t chunk_start[kMaxChunks];
@@ -376,20 +417,30 @@ struct ExpertParams {
   uint32_t* status;
 };
 
-__host__ __device__ inline long long first_unit(long long c, long long total, long long parts) { return c * total / parts; }
-__device__ __forceinline__ int cta_of_unit(long long u, long long total, long long parts) {
-  return static_cast<int>(((u + 1) * parts - 1) / total);
-}
+// `total` units cut evenly over `parts` CTAs, each of which has at least one.
+struct Shares {
+  uint32_t total, parts, base, extra;                  // the first `extra` CTAs have base + 1 units
+  __device__ __forceinline__ Shares(uint32_t total_, uint32_t ctas) : total(total_), parts(min(total_, ctas)) {
+    base = parts > 0 ? total / parts : 0u;
+    extra = total - base * parts;
+  }
+  __device__ __forceinline__ uint32_t first(uint32_t c) const { return c < parts ? c * base + min(c, extra) : total; }
+  __device__ __forceinline__ uint32_t cta_of(uint32_t u) const {
+    const uint32_t large = extra * (base + 1);
+    return u < large ? u / (base + 1) : extra + (u - large) / base;
+  }
+};
 
 // Position in the unit list of a phase.  gate/up: (chunk, pair of 128 outputs, K block); down: (256 output rows, chunk, K block).
 struct Cursor {
   int chunk, j, g, groups, chunks, pairs, phase;
-  __device__ __forceinline__ Cursor(int phase_, long long u, int chunks_, int pairs_, int groups_)
+  __device__ __forceinline__ Cursor(int phase_, uint32_t u, int chunks_, int pairs_, int groups_)
       : groups(groups_), chunks(chunks_), pairs(pairs_), phase(phase_) {
-    const long long item = u / groups;
+    const uint32_t item = u / static_cast<uint32_t>(groups), inner = static_cast<uint32_t>(phase == 0 ? pairs : chunks);
     g = static_cast<int>(u - item * groups);
-    if (phase == 0) { chunk = static_cast<int>(item / pairs); j = static_cast<int>(item % pairs); }
-    else { j = static_cast<int>(item / max(chunks, 1)); chunk = static_cast<int>(item % max(chunks, 1)); }
+    const int outer = static_cast<int>(item / inner), within = static_cast<int>(item % inner);
+    chunk = phase == 0 ? outer : within;
+    j = phase == 0 ? within : outer;
   }
   __device__ __forceinline__ void next() {
     if (++g < groups) return;
@@ -438,7 +489,7 @@ __device__ __forceinline__ void build_work_list(const ExpertParams& p, Tail* tai
     for (int t = warp; t < p.t; t += kWarps) {
       int id;
       float w;
-      topk_token(p.scores + static_cast<int64_t>(t) * p.experts, p.experts, p.k, p.rule, lane, id, w);
+      topk_any(p.scores + static_cast<int64_t>(t) * p.experts, p.experts, p.k, p.rule, lane, id, w);
       if (lane < p.k) {
         rt.slot_expert[t * p.k + lane] = static_cast<int16_t>(id);
         if (blockIdx.x == 0) {
@@ -465,7 +516,7 @@ __device__ __forceinline__ void build_work_list(const ExpertParams& p, Tail* tai
       const int before = __popc(same & ((1u << lane) - 1u));
       const int have = e >= 0 ? rt.count[e] : 0;
       __syncwarp();
-      if (s < slots) tail->pos_of_slot[s] = static_cast<uint16_t>(e >= 0 ? have + before : 0xffff);
+      if (s < slots) tail->place_of_slot[s] = static_cast<uint16_t>(e >= 0 ? have + before : 0xffff);
       if (e >= 0 && (same >> lane) == 1u) rt.count[e] = static_cast<uint16_t>(have + before + 1);   // the last of them
       __syncwarp();
     }
@@ -481,7 +532,7 @@ __device__ __forceinline__ void build_work_list(const ExpertParams& p, Tail* tai
         if (lane >= o) { upto += a; chunks_upto += b; }
       }
       const int first = pos + upto - c;
-      if (e < p.experts) rt.start[e] = static_cast<uint16_t>(first);
+      if (e < p.experts) { rt.start[e] = static_cast<uint16_t>(first); rt.chunk[e] = static_cast<uint16_t>(chunk + chunks_upto - n); }
       for (int q = 0; q < n; ++q) {
         const int at = chunk + chunks_upto - n + q;
         tail->chunk_expert[at] = static_cast<uint16_t>(e);
@@ -497,9 +548,9 @@ __device__ __forceinline__ void build_work_list(const ExpertParams& p, Tail* tai
   for (int s = threadIdx.x; s < slots; s += kThreads) {
     const int e = rt.slot_expert[s];
     if (e >= 0) {
-      const int pos = rt.start[e] + tail->pos_of_slot[s];
-      tail->pos_of_slot[s] = static_cast<uint16_t>(pos);
-      tail->token_of_pos[pos] = static_cast<uint8_t>(s / p.k);
+      const int at = tail->place_of_slot[s];
+      tail->place_of_slot[s] = static_cast<uint16_t>((rt.chunk[e] + at / NC) * 64 + at % NC);
+      tail->token_of_pos[rt.start[e] + at] = static_cast<uint8_t>(s / p.k);
     }
   }
   __syncthreads();
@@ -530,6 +581,14 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
     tail->abort_flag = 0;
     ptx::fence_mbar_init();
   }
+  if (threadIdx.x == kRowProducer * 32) {
+    ptx::prefetch_tensormap(&tmap_w13);
+    ptx::prefetch_tensormap(&tmap_w2);
+  }
+  if (threadIdx.x == kTokenProducer * 32) {
+    ptx::prefetch_tensormap(&tmap_x);
+    ptx::prefetch_tensormap(&tmap_h);
+  }
   if (warp == kIssuer) {
     ptx::tmem_alloc(ptx::smem_u32(&tail->tmem_base), C::kTmemCols);
     ptx::tmem_relinquish();
@@ -541,11 +600,9 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = tail->tmem_base;
   const int chunks = tail->chunks;
-  const long long total[2] = {static_cast<long long>(chunks) * p.gi * p.gh, static_cast<long long>(p.hpairs) * chunks * p.gi};
-  // the CTAs that share a phase's units: each of them has at least one
-  const long long parts[2] = {min(total[0], static_cast<long long>(gridDim.x)), min(total[1], static_cast<long long>(gridDim.x))};
-  auto unit = [&](int phase, int c) { return c < parts[phase] ? first_unit(c, total[phase], parts[phase]) : total[phase]; };
-  auto cursor = [&](int phase, long long u) {
+  const Shares shares[2] = {Shares(static_cast<uint32_t>(chunks) * p.gi * p.gh, gridDim.x),
+                            Shares(static_cast<uint32_t>(p.hpairs) * chunks * p.gi, gridDim.x)};
+  auto cursor = [&](int phase, uint32_t u) {
     return phase == 0 ? Cursor(0, u, chunks, p.gi, p.gh) : Cursor(1, u, chunks, p.hpairs, p.gi);
   };
   const uint32_t barrier_count = 2u * gridDim.x;                   // both tile halves of every CTA arrive
@@ -557,10 +614,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
       uint32_t stage = 0, parity = 0;
       bool ok = true;
       for (int phase = 0; phase < 2 && ok; ++phase) {
-        const long long u0 = unit(phase, blockIdx.x), u1 = unit(phase, blockIdx.x + 1);
+        const uint32_t u0 = shares[phase].first(blockIdx.x), u1 = shares[phase].first(blockIdx.x + 1);
         if (u0 >= u1) continue;
         Cursor c = cursor(phase, u0);
-        for (long long u = u0; u < u1; ++u, c.next()) {
+        for (uint32_t u = u0; u < u1; ++u, c.next()) {
           const uint32_t full = ptx::smem_u32(&tail->full[stage]), dst = smem_base + stage * C::kStageBytes;
           ok = ptx::mbar_wait(ptx::smem_u32(&tail->empty[stage]), parity ^ 1u, abort_flag, p.wait_limit);
           if (!ok) break;
@@ -584,7 +641,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
     uint32_t stage = 0, parity = 0;
     bool ok = true;
     for (int phase = 0; phase < 2 && ok; ++phase) {
-      const long long u0 = unit(phase, blockIdx.x), u1 = unit(phase, blockIdx.x + 1);
+      const uint32_t u0 = shares[phase].first(blockIdx.x), u1 = shares[phase].first(blockIdx.x + 1);
       if (u0 >= u1) continue;
       if (phase == 1) {
         bool there = true;
@@ -593,7 +650,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
         fence_proxy_async();                                       // h was written by ordinary stores, TMA reads it
       }
       Cursor c = cursor(phase, u0);
-      for (long long u = u0; u < u1; ++u, c.next()) {
+      for (uint32_t u = u0; u < u1; ++u, c.next()) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->empty[stage]), parity ^ 1u, abort_flag, p.wait_limit));
         if (!ok) break;
         const uint32_t full = ptx::smem_u32(&tail->full[stage]), dst = smem_base + stage * C::kStageBytes + kWBytes;
@@ -620,10 +677,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
       uint32_t stage = 0, parity = 0, kb = 0;
       bool ok = true;
       for (int phase = 0; phase < 2 && ok; ++phase) {
-        const long long u0 = unit(phase, blockIdx.x), u1 = unit(phase, blockIdx.x + 1);
+        const uint32_t u0 = shares[phase].first(blockIdx.x), u1 = shares[phase].first(blockIdx.x + 1);
         if (u0 >= u1) continue;
         Cursor c = cursor(phase, u0);
-        for (long long u = u0; u < u1; ++u, ++kb, c.next()) {
+        for (uint32_t u = u0; u < u1; ++u, ++kb, c.next()) {
           const uint32_t buf = kb % kAccBufs, acc_parity = (kb / kAccBufs) & 1u;
           ok = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_empty[tile][buf]), acc_parity ^ 1u, abort_flag, p.wait_limit) &&
                ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit);
@@ -649,7 +706,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
     uint32_t kb = 0;
     bool ok = true;
     for (int phase = 0; phase < 2 && ok; ++phase) {
-      const long long u0 = unit(phase, blockIdx.x), u1 = unit(phase, blockIdx.x + 1);
+      const uint32_t u0 = shares[phase].first(blockIdx.x), u1 = shares[phase].first(blockIdx.x + 1);
       if (u0 >= u1) continue;
       if (phase == 1) {
         bool there = true;
@@ -682,7 +739,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
 #pragma unroll
       for (int i = 0; i < kScaleAhead; ++i)
         if (u0 + i < u1) fetch(va[i], vw[i]);
-      for (long long base = u0; base < u1 && ok; base += kScaleAhead) {
+      for (uint32_t base = u0; base < u1 && ok; base += kScaleAhead) {
 #pragma unroll
         for (int i = 0; i < kScaleAhead; ++i) {
           if (base + i < u1 && ok) {
@@ -719,49 +776,61 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
     uint32_t kb = 0;
     bool ok = true;
     for (int phase = 0; phase < 2; ++phase) {
-      const long long u0 = unit(phase, blockIdx.x), u1 = unit(phase, blockIdx.x + 1);
+      const uint32_t u0 = shares[phase].first(blockIdx.x), u1 = shares[phase].first(blockIdx.x + 1);
       if (u0 < u1) {
         Cursor c = cursor(phase, u0);
-        long long seg_start = u0;
-        auto segment_end = [&](long long u, bool alive) {
+        uint32_t seg_start = u0;
+        auto segment_end = [&](uint32_t u, bool alive) {
           const int pos = tail->chunk_start[c.chunk], n = tail->chunk_count[c.chunk];
-          const long long item_first = u - c.g;
-          const int c_first = cta_of_unit(item_first, total[phase], parts[phase]);
-          const int c_last = cta_of_unit(item_first + c.groups - 1, total[phase], parts[phase]);
+          const uint32_t item_first = u - c.g;
+          const int c_first = static_cast<int>(shares[phase].cta_of(item_first));
+          const int c_last = static_cast<int>(shares[phase].cta_of(item_first + c.groups - 1));
           uint32_t* flags = p.sync + kSyncFlags + phase * kMaxGrid * 2;
           bool finish = alive;
           if (seg_start != item_first) {
             // The item's first CTA finishes it: this one hands its sums over (an item that began before this CTA's range is
-            // the first thing in it, so there is one such partial per CTA and phase) and counts itself in.
+            // the first thing in it, so there is one such partial per CTA and phase).  In the second phase they are added
+            // behind the grid barrier, by whoever sums the token.
             float* dst = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + tile) * (NC * 128) + row;
 #pragma unroll
             for (int j = 0; j < NC; ++j)
               if (j < n) __stcg(dst + j * 128, acc[j]);
-            __threadfence();
-            named_sync(1 + tile, 128);
-            if (tid == 0) red_release_add(flags + blockIdx.x * 2 + tile);
-            finish = false;
-          } else if (c_last != c_first) {
-            // Its own part is the last thing in its range; the others' partials are added in the order of the K range,
-            // whatever the timing.
-            if (tid == 0) {
-              bool there = true;
-              for (int o = c_first + 1; o <= c_last && there; ++o)
-                there = wait_word(flags + o * 2 + tile, 1u, abort_flag, p.wait_limit);
-              tail->flag[tile] = there ? 1u : 0u;
+            if (phase == 0) {
+              named_sync(1 + tile, 128);
+              if (tid == 0) red_release_add(flags + blockIdx.x * 2 + tile);
             }
+            finish = false;
+          } else if (phase == 0 && c_last != c_first) {
+            // Its own part is the last thing in its range; the others' partials are added in the order of the K range,
+            // whatever the timing.  One thread waits for each of the others.
+            if (tid == 0) tail->flag[tile] = 1u;
             named_sync(1 + tile, 128);
-            finish = finish && tail->flag[tile] != 0;
-            if (tail->flag[tile] != 0) {
-              __threadfence();
-              for (int o = c_first + 1; o <= c_last; ++o) {
-                const float* src = p.partials + (static_cast<int64_t>(o) * 2 + tile) * (NC * 128) + row;
+            for (int o = c_first + 1 + tid; o <= c_last; o += 128)
+              if (!wait_word(flags + o * 2 + tile, 1u, abort_flag, p.wait_limit)) tail->flag[tile] = 0u;
+            named_sync(1 + tile, 128);
+            const bool there = tail->flag[tile] != 0;
+            finish = finish && there;
+            if (there) {
+              const int64_t pitch = 2 * NC * 128;
+              const float* src = p.partials + (static_cast<int64_t>(c_first + 1) * 2 + tile) * (NC * 128) + row;
+              for (int o = c_last - c_first; o > 0; o -= 4, src += 4 * pitch) {
+                // four CTAs' sums of four columns on their way at a time
 #pragma unroll
-                for (int j = 0; j < NC; ++j)
-                  if (j < n) acc[j] += __ldcg(src + j * 128);
+                for (int j0 = 0; j0 < NC; j0 += 4) {
+                  if (j0 < n) {
+                    float v[4][4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                      for (int j = 0; j < 4; ++j) v[w][j] = w < o && j0 + j < n ? __ldcg(src + w * pitch + (j0 + j) * 128) : 0.0f;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                      for (int j = 0; j < 4; ++j) acc[j0 + j] += v[w][j];
+                  }
+                }
               }
             }
-            named_sync(1 + tile, 128);                             // flag may be rewritten
           }
           if (seg_start == item_first) {
             if (phase == 0) {
@@ -778,6 +847,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
                   float v[8];
 #pragma unroll
                   for (int j = 0; j < 8; ++j) {
+                    if (q * 16 + tile * 8 + j >= n) { v[j] = 0.0f; continue; }
                     const float other = tail->ex.value[tile][j][row], own = tile == 0 ? acc[q * 16 + j] : acc[q * 16 + 8 + j];
                     v[j] = col < p.i ? (tile == 0 ? silu_mul(own, other) : silu_mul(other, own)) : 0.0f;
                     const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -787,13 +857,14 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
 #pragma unroll
                   for (int j = 0; j < 8; ++j) {
                     const int place = q * 16 + tile * 8 + j;
+                    if (place >= n) continue;
                     uint32_t bits = 0u;                            // as integers: a NaN is the largest
 #pragma unroll
                     for (int w = 0; w < 4; ++w) bits = max(bits, __float_as_uint(tail->ex.most[tile * 4 + w][j]));
                     const float scale = group_scale(bits);
                     const float rcp = __frcp_rn(scale);
                     const uint32_t code = p.half ? quant_half_e4m3x2(v[j], 0.0f, scale, rcp) : quant_e4m3x2(v[j], 0.0f, scale, rcp);
-                    if (finish && place < n) {
+                    if (finish) {
                       if (col < p.i) p.hq[static_cast<int64_t>(pos + place) * p.i + col] = static_cast<uint8_t>(code);
                       if (row == 0) p.h_scales[static_cast<int64_t>(c.j) * p.spad + pos + place] = p.half ? scale * 2.0f : scale;
                     }
@@ -815,7 +886,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
           for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
           seg_start = u + 1;
         };
-        long long u = u0;
+        uint32_t u = u0;
         for (; u < u1; ++u, ++kb) {
           const uint32_t buf = kb % kAccBufs, acc_parity = (kb / kAccBufs) & 1u;
           ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full[tile][buf]), acc_parity, abort_flag, p.wait_limit));
@@ -852,8 +923,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
         }
       }
       // ---- grid barrier: everything this half of the CTA wrote in the phase is visible
-      __threadfence();
-      fence_proxy_async();
+      if (phase == 0) fence_proxy_async();
       named_sync(1 + tile, 128);
       if (tid == 0) red_release_add(p.sync + kSyncBarrier + 32 * phase);
     }
@@ -861,23 +931,61 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
     if (tid == 0) tail->flag[tile] = wait_word(p.sync + kSyncBarrier + 32, barrier_count, abort_flag, p.wait_limit) ? 1u : 0u;
     named_sync(1 + tile, 128);
     if (tail->flag[tile] != 0) {
-      __threadfence();
       const int per_token = (p.h + 127) / 128;                     // a warp takes 128 columns of a token
-      for (long long w = static_cast<long long>(warp) * gridDim.x + blockIdx.x; w < static_cast<long long>(p.t) * per_token;
-           w += 8ll * gridDim.x) {
-        const int t = static_cast<int>(w / per_token), col = static_cast<int>(w % per_token) * 128 + lane * 4;
-        if (col < p.h) {
-          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int j = 0; j < p.k; ++j) {
-            const int pos = tail->pos_of_slot[t * p.k + j];
-            if (pos == 0xffff) continue;
-            const float wt = __ldcg(p.weights + t * p.k + j);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.y + static_cast<int64_t>(pos) * p.h + col));
-            sum.x = fmaf(wt, v.x, sum.x); sum.y = fmaf(wt, v.y, sum.y);
-            sum.z = fmaf(wt, v.z, sum.z); sum.w = fmaf(wt, v.w, sum.w);
+      for (uint32_t w = warp * gridDim.x + blockIdx.x; w < static_cast<uint32_t>(p.t) * per_token; w += 8u * gridDim.x) {
+        const int t = static_cast<int>(w / per_token), block = static_cast<int>(w % per_token), col = block * 128 + lane * 4;
+        // lane j looks up slot j: where its sum lies, and how many more CTAs hold parts of its K range
+        int more = -1;
+        const float *own = nullptr, *parts = nullptr;
+        float weight = 0.0f;
+        if (lane < p.k) {
+          const int place = tail->place_of_slot[t * p.k + lane];
+          if (place != 0xffff) {
+            const int chunk = place >> 6, column = place & 63;
+            const uint32_t u = (static_cast<uint32_t>(block >> 1) * chunks + chunk) * p.gi;
+            const int first = static_cast<int>(shares[1].cta_of(u));
+            more = static_cast<int>(shares[1].cta_of(u + p.gi - 1)) - first;
+            own = p.y + static_cast<int64_t>(tail->chunk_start[chunk] + column) * p.h + block * 128;
+            parts = p.partials + ((static_cast<int64_t>(first + 1) * 2 + (block & 1)) * NC + column) * 128;
+            weight = __ldcg(p.weights + t * p.k + lane);
           }
-          *reinterpret_cast<uint2*>(p.out + t * p.ldo + col) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
         }
+        const int deepest = __reduce_max_sync(0xffffffffu, more);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j0 = 0; j0 < p.k; j0 += 4) {                      // four slots' loads on their way at a time
+          float4 v[4];
+          const float* at[4];
+          int n[4];
+          float wt[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int from = min(j0 + j, 31);
+            const unsigned long long a = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(own), from);
+            at[j] = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(parts), from));
+            n[j] = __shfl_sync(0xffffffffu, more, from);
+            wt[j] = __shfl_sync(0xffffffffu, weight, from);
+            if (j0 + j >= p.k || col >= p.h) n[j] = -1;
+            v[j] = n[j] >= 0 ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a) + lane * 4))
+                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+          for (int o = 0; o < deepest; ++o) {
+            float4 a[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              a[j] = o < n[j] ? __ldcg(reinterpret_cast<const float4*>(at[j] + static_cast<int64_t>(o) * (2 * NC * 128) + lane * 4))
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { v[j].x += a[j].x; v[j].y += a[j].y; v[j].z += a[j].z; v[j].w += a[j].w; }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n[j] >= 0) {
+              sum.x = fmaf(wt[j], v[j].x, sum.x); sum.y = fmaf(wt[j], v[j].y, sum.y);
+              sum.z = fmaf(wt[j], v[j].z, sum.z); sum.w = fmaf(wt[j], v[j].w, sum.w);
+            }
+        }
+        if (col < p.h)
+          *reinterpret_cast<uint2*>(p.out + t * p.ldo + col) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
       }
     }
   }
@@ -934,11 +1042,13 @@ int launch_experts(const CUtensorMap& w13, const CUtensorMap& w2, const CUtensor
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   // the CTAs wait for one another: the launch has to put all of them on the device together
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeCooperative;
   attr[0].val.cooperative = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, moe_experts_kernel<NC>, w13, w2, x, hm, p));
   return BFP8_OK;
 }
@@ -956,7 +1066,7 @@ int moe_layer(const uint16_t* x, int64_t ldx, const Router* router, const int32_
               size_t workspace_bytes, uint32_t* status_dev, void* stream, int max_ctas, int64_t wait_limit_cycles) {
   if (!x || !w13 || !s13 || !w2 || !s2 || !out || !status_dev || !workspace) return BFP8_ERR_NULL;
   if (router ? !router->weight : (!ids || !weights)) return BFP8_ERR_NULL;
-  if (t <= 0 || k <= 0 || e <= 0 || h <= 0 || i <= 0 || h > (1 << 20) || i > (1 << 20) || ldx < h || ldo < h) return BFP8_ERR_SHAPE;
+  if (t <= 0 || k <= 0 || e <= 0 || h <= 0 || i <= 0 || h > kMaxWidth || i > kMaxWidth || ldx < h || ldo < h) return BFP8_ERR_SHAPE;
   if (t > kMaxTokens || k > kMaxTopK || e > kMaxExperts || t * k > kMaxSlots || h % 16 != 0 || i % 16 != 0)
     return BFP8_ERR_UNSUPPORTED;
   if (router && (k > e || router->ld < h)) return BFP8_ERR_SHAPE;
@@ -1076,7 +1186,7 @@ extern "C" int bfp8_moe_route(const uint16_t* x, int64_t ldx, const uint16_t* ro
 
 extern "C" size_t bfp8_moe_block128_workspace_bytes(int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t inter) {
   if (t <= 0 || top_k <= 0 || experts <= 0 || h <= 0 || inter <= 0 || t > kMaxTokens || t * top_k > kMaxSlots ||
-      experts > kMaxExperts || h > (1 << 20) || inter > (1 << 20))
+      experts > kMaxExperts || h > kMaxWidth || inter > kMaxWidth)
     return 0;
   return layout_of(t, top_k, experts, h, inter).bytes;
 }

@@ -12,7 +12,7 @@ from . import _lib
 from .block_fp8_gemm import _WAIT_TIMEOUT_MSG
 from .fp8_codec import BLOCK, _device_guard, _empty, _read_status, _status_buffer, _stream_ptr, _unread_status_buffer
 
-MAX_TOKENS, MAX_TOP_K, MAX_SLOTS, MAX_EXPERTS = 128, 32, 2048, 512
+MAX_TOKENS, MAX_TOP_K, MAX_SLOTS, MAX_EXPERTS, MAX_WIDTH = 128, 32, 2048, 512, 1 << 16
 _SCORING = {"softmax": 0, "sigmoid": 1}
 _E4M3 = (torch.float8_e4m3fn, torch.uint8)
 
@@ -88,8 +88,8 @@ def _check_experts(x, top_k, w_gate_up, s_gate_up, w_down, s_down, out):
         if (not isinstance(s, torch.Tensor) or s.dtype != torch.float32 or tuple(s.shape) != shape or not s.is_contiguous()
                 or s.device != x.device):
             raise ValueError("%s must be contiguous FP32 %s on x's device" % (name, shape))
-    if h % 16 or inter % 16:
-        raise ValueError("H and I must be multiples of 16")
+    if h % 16 or inter % 16 or h > MAX_WIDTH or inter > MAX_WIDTH:
+        raise ValueError("H and I must be multiples of 16 and at most %d" % MAX_WIDTH)
     if t > MAX_TOKENS or top_k > MAX_TOP_K or t * top_k > MAX_SLOTS or experts > MAX_EXPERTS:
         raise ValueError("at most %d tokens, %d choices per token, %d in all and %d experts"
                          % (MAX_TOKENS, MAX_TOP_K, MAX_SLOTS, MAX_EXPERTS))

@@ -355,7 +355,7 @@ int bfp8_moe_route(const uint16_t* x, int64_t ldx, const uint16_t* router, int64
  *   ids int32 [t, top_k]: a negative one adds nothing (an expert of another GPU); one beyond the last expert adds
  *   nothing either and raises BFP8_STATUS_BAD_INDEX.  An expert may occur several times in a token.
  *   out bf16 [t, h], row stride ldo (ldo % 4 == 0, 8-byte aligned); x bf16 [t, h], row stride ldx
- * t <= 128, top_k <= 32, t * top_k <= 2048, experts <= 512, h and inter multiples of 16 (BFP8_ERR_UNSUPPORTED otherwise);
+ * t <= 128, top_k <= 32, t * top_k <= 2048, experts <= 512, h and inter multiples of 16 (BFP8_ERR_UNSUPPORTED otherwise) and <= 65536;
  * weights 16-byte aligned and contiguous.  workspace: bfp8_moe_block128_workspace_bytes() bytes, 256-byte aligned, in any
  * state; calls that may overlap on the device need separate ones.  The second kernel is launched cooperatively on all
  * SMs.  max_ctas / wait_limit_cycles: as bfp8_gemm_block128_ex.  status |= WAIT_TIMEOUT if an internal wait gave up; the
