@@ -150,7 +150,7 @@ moe_topk_kernel(const float* __restrict__ scores, int64_t tokens, int experts, i
 // ---------------------------------------------------------------------------------------------------------------------
 // First kernel: router scores and activation quantizer
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kFrontWarps = 8;
+constexpr int kFrontWarps = 16;
 
 struct FrontParams {
   const uint16_t* x;
@@ -233,7 +233,7 @@ __device__ __forceinline__ void router_tile(const FrontParams& p, int64_t t0, in
   const uint4 none = make_uint4(0u, 0u, 0u, 0u);
   const uint16_t *r0 = p.router + static_cast<int64_t>(e0 + g) * p.ldr, *r1 = r0 + 8 * p.ldr;
   const bool has0 = e0 + g < p.experts, has1 = e0 + g + 8 < p.experts;
-#pragma unroll 2
+#pragma unroll 4
   for (int c = warp * 32; c < p.h; c += kFrontWarps * 32) {
     const int k = c + t * 8;
     const uint4 w0 = has0 ? load8(r0, k, p.h, vec) : none, w1 = has1 ? load8(r1, k, p.h, vec) : none;
@@ -331,7 +331,7 @@ moe_front_kernel(const FrontParams p) {
 int launch_front(FrontParams& p, cudaStream_t st) {
   const int64_t quant = p.quant_blocks ? (p.t * p.groups + kFrontWarps - 1) / kFrontWarps : 0;
   p.quant_blocks = static_cast<int>(quant);
-  const int columns = p.t <= 4 ? 0 : p.t <= 8 ? 1 : p.t <= 16 ? 2 : 4;
+  const int columns = p.t <= 4 ? 0 : p.t <= 8 ? 1 : 2;
   int64_t route = 0;
   if (p.router != nullptr)
     route = columns == 0 ? (p.t * p.experts + kFrontWarps - 1) / kFrontWarps
@@ -341,8 +341,7 @@ int launch_front(FrontParams& p, cudaStream_t st) {
   switch (columns) {
     case 0: return launch_overlapped(moe_front_kernel<0>, grid, block, 0, st, p);
     case 1: return launch_overlapped(moe_front_kernel<1>, grid, block, 0, st, p);
-    case 2: return launch_overlapped(moe_front_kernel<2>, grid, block, 0, st, p);
-    default: return launch_overlapped(moe_front_kernel<4>, grid, block, 0, st, p);
+    default: return launch_overlapped(moe_front_kernel<2>, grid, block, 0, st, p);
   }
 }
 
@@ -968,14 +967,18 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
             v[j] = n[j] >= 0 ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a) + lane * 4))
                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           }
-          for (int o = 0; o < deepest; ++o) {
-            float4 a[4];
+          for (int o = 0; o < deepest; o += 3) {
+            float4 a[3][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              a[j] = o < n[j] ? __ldcg(reinterpret_cast<const float4*>(at[j] + static_cast<int64_t>(o) * (2 * NC * 128) + lane * 4))
-                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int i = 0; i < 3; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { v[j].x += a[j].x; v[j].y += a[j].y; v[j].z += a[j].z; v[j].w += a[j].w; }
+              for (int j = 0; j < 4; ++j)
+                a[i][j] = o + i < n[j] ? __ldcg(reinterpret_cast<const float4*>(at[j] + static_cast<int64_t>(o + i) * (2 * NC * 128) + lane * 4))
+                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) { v[j].x += a[i][j].x; v[j].y += a[i][j].y; v[j].z += a[i][j].z; v[j].w += a[i][j].w; }
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)

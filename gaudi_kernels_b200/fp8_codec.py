@@ -76,6 +76,20 @@ def _unread_status_buffer(device):
     return torch.empty_strided((4,), (1,), dtype=torch.int32, device=device)
 
 
+_sinks = {}
+
+
+def _status_sink(dev):
+    """A status buffer that nobody reads, one per device and kept: kernels only ever set bits in it.  A call that is being
+    captured allocates one of its own rather than keep memory of the graph's pool (and a tensor without memory is not kept)."""
+    sink = _sinks.get(dev)
+    if sink is None:
+        sink = _unread_status_buffer(dev)
+        if sink.data_ptr() and not torch.cuda.is_current_stream_capturing():
+            _sinks[dev] = sink
+    return sink
+
+
 def _read_status(buf):
     lo, hi, status = buf.tolist()[:3]      # synchronises with the launching stream; a caller's buffer may be longer
     return ((hi & 0xFFFFFFFF) << 32) | (lo & 0xFFFFFFFF), status & 0xFFFFFFFF

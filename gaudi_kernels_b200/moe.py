@@ -6,30 +6,43 @@ the routing is: the router's products with the activation quantizer, and the exp
 reference has no mixture-of-experts kernels.
 """
 
+import functools
+
 import torch
 
 from . import _lib
 from .block_fp8_gemm import _WAIT_TIMEOUT_MSG
-from .fp8_codec import BLOCK, _device_guard, _empty, _read_status, _status_buffer, _stream_ptr, _unread_status_buffer
+from .fp8_codec import BLOCK, _device_guard, _empty, _read_status, _status_buffer, _status_sink, _stream_ptr
 
 MAX_TOKENS, MAX_TOP_K, MAX_SLOTS, MAX_EXPERTS, MAX_WIDTH = 128, 32, 2048, 512, 1 << 16
 _SCORING = {"softmax": 0, "sigmoid": 1}
 _E4M3 = (torch.float8_e4m3fn, torch.uint8)
+_BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(t, k, experts, h, inter):
+    """A pure function of the sizes; the C call takes longer than looking it up."""
+    return _lib.load().bfp8_moe_block128_workspace_bytes(t, k, experts, h, inter)
+
+
+# A decode step's calls are bound by the host where the batch is small, so the checks below touch each property once and
+# build their messages only when they fail.
 
 def _check_rows(x):
-    if (not isinstance(x, torch.Tensor) or x.dtype != torch.bfloat16 or x.ndim != 2 or x.shape[1] < 1
-            or (x.shape[1] > 1 and x.stride(1) != 1) or x.device.type != "cuda"):
+    if (not isinstance(x, torch.Tensor) or x.dtype != _BF16 or x.ndim != 2 or not x.is_cuda or x.shape[1] < 1
+            or (x.stride(1) != 1 and x.shape[1] > 1)):
         raise ValueError("x must be a bf16 [T, H] CUDA tensor with unit column stride")
 
 
-def _check_router(x, router_weight, top_k, scoring, bias):
-    """Checked arguments of a router: (bias or None, number of experts)."""
-    if (not isinstance(router_weight, torch.Tensor) or router_weight.dtype != torch.bfloat16 or router_weight.ndim != 2
-            or router_weight.shape[1] != x.shape[1] or router_weight.shape[0] < 1
-            or (x.shape[1] > 1 and router_weight.stride(1) != 1) or router_weight.device != x.device):
-        raise ValueError("router_weight must be bf16 [E, H] with unit column stride on x's device")
-    experts = router_weight.shape[0]
+def _check_router(dev, h, router_weight, top_k, scoring, bias):
+    """Checked arguments of a router: the number of experts."""
+    if (not isinstance(router_weight, torch.Tensor) or router_weight.dtype != _BF16 or router_weight.ndim != 2
+            or router_weight.device != dev):
+        raise ValueError("router_weight must be bf16 [E, H] on x's device")
+    experts, width = router_weight.shape
+    if width != h or experts < 1 or (router_weight.stride(1) != 1 and h > 1):
+        raise ValueError("router_weight must be [E, H] with x's H and unit column stride")
     if scoring not in _SCORING:
         raise ValueError("scoring must be 'softmax' or 'sigmoid'")
     if not 1 <= top_k <= min(experts, MAX_TOP_K) or experts > MAX_EXPERTS:
@@ -37,13 +50,13 @@ def _check_router(x, router_weight, top_k, scoring, bias):
     if bias is not None:
         if scoring != "sigmoid":
             raise ValueError("a bias on the choice goes with sigmoid scoring")
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (experts,) or not bias.is_contiguous() or bias.device != x.device:
+        if bias.dtype != _F32 or bias.shape != (experts,) or not bias.is_contiguous() or bias.device != dev:
             raise ValueError("bias must be contiguous FP32 [E] on x's device")
     return experts
 
 
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _row_stride(t, rows, width):
+    return t.stride(0) if rows > 1 else width
 
 
 def route_topk(x, router_weight, top_k, *, scoring="softmax", renormalize=True, bias=None, scale=1.0):
@@ -55,49 +68,52 @@ def route_topk(x, router_weight, top_k, *, scoring="softmax", renormalize=True, 
     `scale`.  Ties go to the lower index; a NaN ranks last.  x bf16 [T, H], router_weight bf16 [E, H], E <= 512, any T.
     """
     _check_rows(x)
-    experts = _check_router(x, router_weight, top_k, scoring, bias)
     t, h = x.shape
     dev = x.device
+    experts = _check_router(dev, h, router_weight, top_k, scoring, bias)
     lib = _lib.load()
     with _device_guard(dev):
-        ids = _empty(t, top_k, torch.int32, dev)
-        weights = _empty(t, top_k, torch.float32, dev)
+        ids = _empty(t, top_k, _I32, dev)
+        weights = _empty(t, top_k, _F32, dev)
         if t == 0:
             return ids, weights
-        scores = _empty(t, experts, torch.float32, dev)
-        rc = lib.bfp8_moe_route(x.data_ptr(), _row_stride(x), router_weight.data_ptr(), _row_stride(router_weight),
-                                None if bias is None else bias.data_ptr(), t, h, experts, top_k, _SCORING[scoring],
-                                int(bool(renormalize)), scale, ids.data_ptr(), weights.data_ptr(), scores.data_ptr(),
-                                t * experts * 4, _stream_ptr(dev))
-        _lib.check(rc, "bfp8_moe_route")
+        scores = _empty(t, experts, _F32, dev)
+        rc = lib.bfp8_moe_route(x.data_ptr(), _row_stride(x, t, h), router_weight.data_ptr(),
+                                _row_stride(router_weight, experts, h), None if bias is None else bias.data_ptr(), t, h, experts,
+                                top_k, _SCORING[scoring], 1 if renormalize else 0, scale, ids.data_ptr(), weights.data_ptr(),
+                                scores.data_ptr(), t * experts * 4, _stream_ptr(dev))
+        if rc:
+            _lib.check(rc, "bfp8_moe_route")
     return ids, weights
 
 
-def _check_experts(x, top_k, w_gate_up, s_gate_up, w_down, s_down, out):
-    """Checked arguments of the experts: (T, H, E, I)."""
-    t, h = x.shape
-    for name, w, dims in (("w_gate_up", w_gate_up, 4), ("w_down", w_down, 3)):
-        if (not isinstance(w, torch.Tensor) or w.dtype not in _E4M3 or w.ndim != dims or not w.is_contiguous()
-                or w.device != x.device):
-            raise ValueError("%s must be a contiguous %d-D E4M3 tensor on x's device" % (name, dims))
-    experts, two, inter, wh = w_gate_up.shape
-    if two != 2 or wh != h or tuple(w_down.shape) != (experts, h, inter) or experts < 1 or inter < 1:
+def _check_experts(dev, t, h, top_k, w_gate_up, s_gate_up, w_down, s_down, out):
+    """Checked arguments of the experts: (E, I)."""
+    if (not isinstance(w_gate_up, torch.Tensor) or w_gate_up.dtype not in _E4M3 or w_gate_up.ndim != 4
+            or not w_gate_up.is_contiguous() or w_gate_up.device != dev):
+        raise ValueError("w_gate_up must be a contiguous 4-D E4M3 tensor on x's device")
+    if (not isinstance(w_down, torch.Tensor) or w_down.dtype not in _E4M3 or not w_down.is_contiguous()
+            or w_down.device != dev):
+        raise ValueError("w_down must be a contiguous 3-D E4M3 tensor on x's device")
+    experts, two, inter, width = w_gate_up.shape
+    if two != 2 or width != h or w_down.shape != (experts, h, inter) or experts < 1 or inter < 1:
         raise ValueError("w_gate_up [E, 2, I, H] and w_down [E, H, I] must agree with x [T, H]")
     gh, gi = (h + BLOCK - 1) // BLOCK, (inter + BLOCK - 1) // BLOCK
-    for name, s, shape in (("s_gate_up", s_gate_up, (experts, 2, gi, gh)), ("s_down", s_down, (experts, gh, gi))):
-        if (not isinstance(s, torch.Tensor) or s.dtype != torch.float32 or tuple(s.shape) != shape or not s.is_contiguous()
-                or s.device != x.device):
-            raise ValueError("%s must be contiguous FP32 %s on x's device" % (name, shape))
+    if (not isinstance(s_gate_up, torch.Tensor) or s_gate_up.dtype != _F32 or s_gate_up.shape != (experts, 2, gi, gh)
+            or not s_gate_up.is_contiguous() or s_gate_up.device != dev):
+        raise ValueError("s_gate_up must be contiguous FP32 %s on x's device" % ((experts, 2, gi, gh),))
+    if (not isinstance(s_down, torch.Tensor) or s_down.dtype != _F32 or s_down.shape != (experts, gh, gi)
+            or not s_down.is_contiguous() or s_down.device != dev):
+        raise ValueError("s_down must be contiguous FP32 %s on x's device" % ((experts, gh, gi),))
     if h % 16 or inter % 16 or h > MAX_WIDTH or inter > MAX_WIDTH:
         raise ValueError("H and I must be multiples of 16 and at most %d" % MAX_WIDTH)
     if t > MAX_TOKENS or top_k > MAX_TOP_K or t * top_k > MAX_SLOTS or experts > MAX_EXPERTS:
         raise ValueError("at most %d tokens, %d choices per token, %d in all and %d experts"
                          % (MAX_TOKENS, MAX_TOP_K, MAX_SLOTS, MAX_EXPERTS))
-    if out is not None and (out.dtype != torch.bfloat16 or tuple(out.shape) != (t, h) or out.stride(1) != 1
-                            or out.device != x.device or (t > 1 and (out.stride(0) < h or out.stride(0) % 4))
-                            or out.data_ptr() % 8):
+    if out is not None and (out.dtype != _BF16 or out.shape != (t, h) or out.stride(1) != 1 or out.device != dev
+                            or (t > 1 and (out.stride(0) < h or out.stride(0) % 4)) or out.data_ptr() % 8):
         raise ValueError("out must be bf16 [T, H] on x's device, rows of unit stride starting on 8-byte boundaries")
-    return t, h, experts, inter
+    return experts, inter
 
 
 def _raise_for(status):
@@ -121,29 +137,33 @@ def moe_block_fp8(x, ids, weights, w_gate_up, s_gate_up, w_down, s_down, *, nati
     wait_limit_cycles as in gemm_block_fp8.  Calls need no workspace of the caller's and may overlap.
     """
     _check_rows(x)
-    if (not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.ndim != 2 or ids.shape[0] != x.shape[0]
-            or ids.shape[1] < 1 or not ids.is_contiguous() or ids.device != x.device):
-        raise ValueError("ids must be contiguous INT32 [T, k] on x's device")
-    if (not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or weights.shape != ids.shape
-            or not weights.is_contiguous() or weights.device != x.device):
-        raise ValueError("weights must be contiguous FP32 [T, k] on x's device")
-    k = ids.shape[1]
-    t, h, experts, inter = _check_experts(x, k, w_gate_up, s_gate_up, w_down, s_down, out)
+    t, h = x.shape
     dev = x.device
+    if (not isinstance(ids, torch.Tensor) or ids.dtype != _I32 or ids.ndim != 2 or not ids.is_contiguous()
+            or ids.device != dev):
+        raise ValueError("ids must be contiguous INT32 [T, k] on x's device")
+    rows, k = ids.shape
+    if rows != t or k < 1:
+        raise ValueError("ids must be [T, k] with x's T and at least one choice")
+    if (not isinstance(weights, torch.Tensor) or weights.dtype != _F32 or weights.shape != (t, k)
+            or not weights.is_contiguous() or weights.device != dev):
+        raise ValueError("weights must be contiguous FP32 [T, k] on x's device")
+    experts, inter = _check_experts(dev, t, h, k, w_gate_up, s_gate_up, w_down, s_down, out)
     lib = _lib.load()
     with _device_guard(dev):
         if out is None:
-            out = _empty(t, h, torch.bfloat16, dev)
+            out = _empty(t, h, _BF16, dev)
         if t == 0:
             return out
-        nbytes = lib.bfp8_moe_block128_workspace_bytes(t, k, experts, h, inter)
-        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=dev)
-        st = status if status is not None else _status_buffer(dev) if check else _unread_status_buffer(dev)
-        rc = lib.bfp8_moe_block128(x.data_ptr(), _row_stride(x), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(),
+        nbytes = _workspace_bytes(t, k, experts, h, inter)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=_U8, device=dev)
+        st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
+        rc = lib.bfp8_moe_block128(x.data_ptr(), _row_stride(x, t, h), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(),
                                    s_gate_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(), out.data_ptr(),
-                                   _row_stride(out), t, k, experts, h, inter, int(bool(native_half)), ws.data_ptr(), nbytes,
+                                   _row_stride(out, t, h), t, k, experts, h, inter, 1 if native_half else 0, ws.data_ptr(), nbytes,
                                    st.data_ptr() + 8, _stream_ptr(dev), max_ctas, wait_limit_cycles)
-        _lib.check(rc, "bfp8_moe_block128")
+        if rc:
+            _lib.check(rc, "bfp8_moe_block128")
         if check:
             _raise_for(st)
     return out
@@ -153,29 +173,31 @@ def moe_layer_block_fp8(x, router_weight, top_k, w_gate_up, s_gate_up, w_down, s
                         bias=None, scale=1.0, native_half=False, out=None, check=True, status=None):
     """(out bf16 [T, H], ids, weights): route_topk and moe_block_fp8 on its choice as two kernels, the same bits."""
     _check_rows(x)
-    if router_weight.shape[0] != w_gate_up.shape[0]:
-        raise ValueError("router_weight [E, H] and w_gate_up [E, 2, I, H] must share E")
-    experts = _check_router(x, router_weight, top_k, scoring, bias)
-    t, h, experts, inter = _check_experts(x, top_k, w_gate_up, s_gate_up, w_down, s_down, out)
+    t, h = x.shape
     dev = x.device
+    experts = _check_router(dev, h, router_weight, top_k, scoring, bias)
+    held, inter = _check_experts(dev, t, h, top_k, w_gate_up, s_gate_up, w_down, s_down, out)
+    if held != experts:
+        raise ValueError("router_weight [E, H] and w_gate_up [E, 2, I, H] must share E")
     lib = _lib.load()
     with _device_guard(dev):
         if out is None:
-            out = _empty(t, h, torch.bfloat16, dev)
-        ids = _empty(t, top_k, torch.int32, dev)
-        weights = _empty(t, top_k, torch.float32, dev)
+            out = _empty(t, h, _BF16, dev)
+        ids = _empty(t, top_k, _I32, dev)
+        weights = _empty(t, top_k, _F32, dev)
         if t == 0:
             return out, ids, weights
-        nbytes = lib.bfp8_moe_block128_workspace_bytes(t, top_k, experts, h, inter)
-        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=dev)
-        st = status if status is not None else _status_buffer(dev) if check else _unread_status_buffer(dev)
-        rc = lib.bfp8_moe_layer_block128(x.data_ptr(), _row_stride(x), router_weight.data_ptr(), _row_stride(router_weight),
-                                         None if bias is None else bias.data_ptr(), _SCORING[scoring], int(bool(renormalize)),
-                                         scale, ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(),
-                                         s_gate_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(), out.data_ptr(),
-                                         _row_stride(out), t, top_k, experts, h, inter, int(bool(native_half)), ws.data_ptr(),
-                                         nbytes, st.data_ptr() + 8, _stream_ptr(dev))
-        _lib.check(rc, "bfp8_moe_layer_block128")
+        nbytes = _workspace_bytes(t, top_k, experts, h, inter)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=_U8, device=dev)
+        st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
+        rc = lib.bfp8_moe_layer_block128(x.data_ptr(), _row_stride(x, t, h), router_weight.data_ptr(),
+                                         _row_stride(router_weight, experts, h), None if bias is None else bias.data_ptr(),
+                                         _SCORING[scoring], 1 if renormalize else 0, scale, ids.data_ptr(), weights.data_ptr(),
+                                         w_gate_up.data_ptr(), s_gate_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(),
+                                         out.data_ptr(), _row_stride(out, t, h), t, top_k, experts, h, inter,
+                                         1 if native_half else 0, ws.data_ptr(), nbytes, st.data_ptr() + 8, _stream_ptr(dev))
+        if rc:
+            _lib.check(rc, "bfp8_moe_layer_block128")
         if check:
             _raise_for(st)
     return out, ids, weights

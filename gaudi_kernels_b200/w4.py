@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from .block_fp8_gemm import _WAIT_TIMEOUT_MSG
-from .fp8_codec import _device_for, _device_guard, _empty, _read_status, _status_buffer, _stream_ptr, _unread_status_buffer
+from .fp8_codec import _device_for, _device_guard, _empty, _read_status, _status_buffer, _status_sink, _stream_ptr
 
 GROUPS = (32, 64, 128)
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1}
@@ -56,17 +56,19 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
     check  read the status word after the launch (one synchronisation) and raise if a bounded wait expired; status as in
            gemm_block_fp8.  The kernel waits for nothing but its own copies, so calls are unchecked by default.
     """
-    if (not isinstance(x, torch.Tensor) or x.dtype not in _DTYPE or x.ndim != 2 or x.device.type != "cuda"
-            or (x.shape[1] > 1 and x.stride(1) != 1)):
+    kind = _DTYPE.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if kind is None or x.ndim != 2 or not x.is_cuda or (x.stride(1) != 1 and x.shape[1] > 1):
         raise ValueError("x must be a bf16 or fp16 [M, K] CUDA tensor with unit column stride")
     m, k = x.shape
     dev = x.device
     if group not in GROUPS or k < 32 or k % 32:
         raise ValueError("group must be 32, 64 or 128 and K a multiple of 32")
-    if (not isinstance(codes, torch.Tensor) or codes.dtype != torch.uint8 or codes.ndim != 2 or codes.shape[1] * 2 != k
-            or codes.shape[0] < 1 or not codes.is_contiguous() or codes.device != dev):
+    if (not isinstance(codes, torch.Tensor) or codes.dtype != torch.uint8 or codes.ndim != 2 or not codes.is_contiguous()
+            or codes.device != dev):
         raise ValueError("codes must be contiguous uint8 [N, K / 2] on x's device")
-    n = codes.shape[0]
+    n, packed = codes.shape
+    if packed * 2 != k or n < 1:
+        raise ValueError("codes must be [N, K / 2] with x's K")
     shape = (n, (k + group - 1) // group)
     if (not isinstance(scales, torch.Tensor) or scales.dtype != x.dtype or scales.shape != shape
             or not scales.is_contiguous() or scales.device != dev):
@@ -79,7 +81,7 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
         raise ValueError("bias must be contiguous FP32 [N] on x's device")
     if out_dtype is None:
         out_dtype = x.dtype if out is None else out.dtype
-    if out_dtype not in (x.dtype, torch.float32):
+    if out_dtype != x.dtype and out_dtype != torch.float32:
         raise ValueError("out_dtype must be x's type or float32")
     if out is not None and (out.dtype != out_dtype or out.shape != (m, n) or (n > 1 and out.stride(1) != 1)
                             or (m > 1 and out.stride(0) < n) or out.device != dev):
@@ -92,13 +94,14 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
             return out
         if x.data_ptr() % 16 or (m > 1 and x.stride(0) % 8):
             x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries
-        st = status if status is not None else _status_buffer(dev) if check else _unread_status_buffer(dev)
-        rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, _DTYPE[x.dtype], codes.data_ptr(),
+        st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
+        rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, kind, codes.data_ptr(),
                                     scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
                                     None if bias is None else bias.data_ptr(), out.data_ptr(),
-                                    int(out_dtype == torch.float32), out.stride(0) if m > 1 else n, m, n, k,
+                                    1 if out_dtype == torch.float32 else 0, out.stride(0) if m > 1 else n, m, n, k,
                                     st.data_ptr() + 8, _stream_ptr(dev), wait_limit_cycles)
-        _lib.check(rc, "bfp8_gemm_group_w4")
+        if rc:
+            _lib.check(rc, "bfp8_gemm_group_w4")
         if check and _read_status(st)[1] & _lib.STATUS_WAIT_TIMEOUT:
             raise _lib.Bfp8Error(_WAIT_TIMEOUT_MSG)
     return out
