@@ -29,8 +29,7 @@ bool weights_at_rest();
 namespace {
 
 constexpr long long kDefaultWaitLimit = 2000000000LL;      // about a second
-constexpr int kStageK = 256;                               // k per stage: 128 bytes of a code row
-constexpr int kMaxRows = 256;                              // weight rows per CTA, the largest TMA box
+constexpr int kStageK = 512;                               // k per stage: twice 128 bytes of a code row
 constexpr int kMaxStages = 16;
 constexpr int kSmemBytes = 225 * 1024;
 constexpr int kMaxCluster = 8;
@@ -43,7 +42,6 @@ struct W4Params {
   int64_t ldo;
   int m, n, k, groups;
   int rows;                    // R
-  int slices;                  // warps that share a row range: 2 take a half of each stage's k each
   int stages;                  // ring depth
   int cluster;
   int out_f32;
@@ -122,13 +120,15 @@ __host__ __device__ constexpr int consumers(int nt) { return 15 - nt; }
 constexpr int kThreads = 16 * 32;
 // 16-row weight tiles per warp: with many activation rows two, so that x is read from shared memory once for both
 __host__ __device__ constexpr int tiles(int nt) { return nt >= 4 ? 2 : 1; }
-// Scales are fetched for several steps at once: from the [n, groups] layout one step's scales of a row are 4 to 16 bytes of a
-// 128-byte line, and a warp-wide load costs a cycle per line
-__host__ __device__ constexpr int super_steps(int nt, int shift) { return (shift == 0 ? 2 : 4) / tiles(nt); }
+// Scales are fetched for up to 1024 k at once: from the [n, groups] layout 256 k of a row are 4 to 16 bytes of a 128-byte line,
+// and a warp-wide load costs a cycle per line
+__host__ __device__ constexpr int super_steps(int nt, int shift) { return shift == 0 || tiles(nt) == 2 ? 1 : 2; }
 __host__ __device__ constexpr int step_groups(int shift) { return kStageK >> (5 + shift); }
 __host__ __device__ constexpr int warp_area(int nt, int shift) { return 16 * tiles(nt) * super_steps(nt, shift) * step_groups(shift) * 8; }
 __host__ __device__ constexpr int ring_bytes(int nt, int shift) { return (kSmemBytes - consumers(nt) * warp_area(nt, shift)) & ~1023; }
-__host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * 128 + mp * kStageK * 2; }
+// weight rows per CTA: a TMA box at most, and two stages have to fit
+__host__ __device__ constexpr int max_rows(int nt) { return nt >= 4 ? 192 : 256; }
+__host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * (kStageK / 2) + mp * kStageK * 2; }
 
 // Scales and zero points of kGroups neighbouring groups of one row as they lie in memory, loaded well before they are used
 template <int kGroups>
@@ -148,11 +148,14 @@ struct RawScales {
         s[0] = v.x; s[1] = v.y;
         if (p.zeros != nullptr) z[0] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
       } else {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.scales + at));
-        s[0] = v.x; s[1] = v.y; s[kGroups > 4 ? 2 : 0] = v.z; s[kGroups > 4 ? 3 : 0] = v.w;
-        if (p.zeros != nullptr) {
-          const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.zeros + at));
-          z[0] = u.x; z[kGroups > 4 ? 1 : 0] = u.y;
+#pragma unroll
+        for (int i = 0; i < kGroups / 8; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.scales + at + 8 * i));
+          s[4 * i] = v.x; s[4 * i + 1] = v.y; s[4 * i + 2 < kGroups / 2 ? 4 * i + 2 : 0] = v.z; s[4 * i + 3 < kGroups / 2 ? 4 * i + 3 : 0] = v.w;
+          if (p.zeros != nullptr) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.zeros + at + 8 * i));
+            z[2 * i] = u.x; z[2 * i + 1 < kGroups / 4 ? 2 * i + 1 : 0] = u.y;
+          }
         }
       }
     } else {
@@ -167,8 +170,9 @@ struct RawScales {
   }
 };
 
-// kNT: activation rows / 8; kShift: group = 32 << kShift.
-template <bool kBf16, int kNT, int kShift>
+// kNT: activation rows / 8; kShift: group = 32 << kShift; kSlices: warps that share a row range, 2 take a half of each
+// stage's k each.
+template <bool kBf16, int kNT, int kShift, int kSlices>
 __global__ void __launch_bounds__(kThreads, 1)
 w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Params p) {
   using H = Half16<kBf16>;
@@ -176,7 +180,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   constexpr int kMp = kNT * 8;
   constexpr int kXBytes = kMp * kStageK * 2;
   constexpr int kStepGroups = step_groups(kShift), kSuper = super_steps(kNT, kShift);
-  constexpr int kLaneGroups = kSuper * kStepGroups * kMT / 2;      // 4 or 8: two lanes per row with one tile, one with two
+  constexpr int kLaneGroups = kSuper * kStepGroups * kMT / 2;      // 4, 8 or 16: two lanes per row with one tile, one with two
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
@@ -184,15 +188,14 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   volatile uint32_t* abort_flag = &tail->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.rows / kWarpRows;                            // warps across R
-  const int slices = p.slices;                                     // warps across the k of a stage: 1 or 2
+  constexpr int slices = kSlices;                                  // warps across the k of a stage
   const uint32_t stage_bytes = static_cast<uint32_t>(stage_size(p.rows, kMp));
   const int rank = p.cluster > 1 ? static_cast<int>(blockIdx.x) % p.cluster : 0;
   const int n0 = static_cast<int>(blockIdx.x) / p.cluster * p.rows;
   const int m0 = blockIdx.y * kMp;
   const int all_steps = (p.k + kStageK - 1) / kStageK;
-  // K is cut between pairs of steps, so that a CTA's scales start on the alignment of their loads
-  const int step0 = static_cast<int>(static_cast<long long>((all_steps + 1) / 2) * rank / p.cluster) * 2;
-  const int step1 = min(static_cast<int>(static_cast<long long>((all_steps + 1) / 2) * (rank + 1) / p.cluster) * 2, all_steps);
+  const int step0 = static_cast<int>(static_cast<long long>(all_steps) * rank / p.cluster);
+  const int step1 = static_cast<int>(static_cast<long long>(all_steps) * (rank + 1) / p.cluster);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -233,7 +236,8 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         for (; early < p.stages && step0 + early < step1; ++early) {
           const uint32_t full = ptx::smem_u32(&tail->full[early]);
           ptx::mbar_arrive_expect_tx(full, stage_bytes);
-          ptx::tma_load_2d_hint(smem_base + early * stage_bytes, &tmap_w, full, (step0 + early) * 128, n0, once);
+          for (int h = 0; h < 2; ++h)
+            ptx::tma_load_2d_hint(smem_base + early * stage_bytes + h * p.rows * 128, &tmap_w, full, (step0 + early) * 256 + h * 128, n0, once);
         }
       ptx::griddep_wait();
       for (int s = step0; s < step1; ++s) {
@@ -243,28 +247,31 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         } else {
           if (!ptx::mbar_wait(ptx::smem_u32(&tail->empty[stage]), parity ^ 1u, abort_flag, p.wait_limit)) break;
           ptx::mbar_arrive_expect_tx(full, stage_bytes);
-          ptx::tma_load_2d_hint(dst, &tmap_w, full, s * 128, n0, once);
+          for (int h = 0; h < 2; ++h) ptx::tma_load_2d_hint(dst + h * p.rows * 128, &tmap_w, full, s * 256 + h * 128, n0, once);
         }
 #pragma unroll
         for (int b = 0; b < kStageK / 64; ++b)
-          ptx::tma_load_2d(dst + p.rows * 128 + b * kMp * 128, &tmap_x, full, s * kStageK + b * 64, m0);
+          ptx::tma_load_2d(dst + p.rows * 256 + b * kMp * 128, &tmap_x, full, s * kStageK + b * 64, m0);
         advance();
       }
     }
   } else if (warp >= kConsumers) {
     // ------------------------------------------------------------------ x of 8 rows: pairs (k, k + 4) side by side, once for all consumers
-    const uint32_t first = p.rows * 128 + ((warp - kConsumers) * 8 + xrow) * 128 + ((t ^ xrow) << 4);
+    const uint32_t first = p.rows * 256 + ((warp - kConsumers) * 8 + xrow) * 128 + ((t ^ xrow) << 4);
     for (int s = step0; s < step1; ++s) {
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit))) break;
       uint8_t* at = smem + stage * stage_bytes;
-      uint4 v[kStageK / 32];
 #pragma unroll
-      for (int q = 0; q < kStageK / 32; ++q) v[q] = *reinterpret_cast<const uint4*>(at + (first ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128));
+      for (int h = 0; h < kStageK / 256; ++h) {
+        uint4 v[8];
 #pragma unroll
-      for (int q = 0; q < kStageK / 32; ++q)
-        *reinterpret_cast<uint4*>(at + (first ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128)) =
-            make_uint4(__byte_perm(v[q].x, v[q].z, 0x5410), __byte_perm(v[q].x, v[q].z, 0x7632),
-                       __byte_perm(v[q].y, v[q].w, 0x5410), __byte_perm(v[q].y, v[q].w, 0x7632));
+        for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const uint4*>(at + (first ^ ((q & 1) << 6)) + (h * 4 + (q >> 1)) * (kMp * 128));
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          *reinterpret_cast<uint4*>(at + (first ^ ((q & 1) << 6)) + (h * 4 + (q >> 1)) * (kMp * 128)) =
+              make_uint4(__byte_perm(v[q].x, v[q].z, 0x5410), __byte_perm(v[q].x, v[q].z, 0x7632),
+                         __byte_perm(v[q].y, v[q].w, 0x5410), __byte_perm(v[q].y, v[q].w, 0x7632));
+      }
       __syncwarp();
       ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->ready[stage]), lane);
       advance();
@@ -275,7 +282,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     // this lane's share of the scales: a row, and with one tile per warp one half of the groups
     const int row = kMT == 1 ? lane & 15 : lane, share = kMT == 1 ? (lane >> 4) * kLaneGroups : 0;
     const uint32_t w_first = unit * kMT * 2048 + g * 128 + (g << 4) + t * 4;      // chunk c of 16 bytes of row r lies at c ^ (r & 7)
-    const uint32_t x_first = p.rows * 128 + xrow * 128 + ((t ^ xrow) << 4);
+    const uint32_t x_first = p.rows * 256 + xrow * 128 + ((t ^ xrow) << 4);
     ptx::griddep_wait();
     RawScales<kLaneGroups> raw;
     raw.load(p, n0 + unit * kWarpRows + row, step0 * kStepGroups + share);
@@ -292,13 +299,15 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
       const int s1 = min(s0 + kSuper, step1);
       bool ok = true;
       for (int s = s0; s < s1; ++s) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit) &&
-                                         ptx::mbar_wait(ptx::smem_u32(&tail->ready[stage]), parity, abort_flag, p.wait_limit));
+        // x is ready: so are the codes, whose copies the x warps waited for
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->ready[stage]), parity, abort_flag, p.wait_limit));
         if (!ok) break;
         const uint8_t* at = smem + stage * stage_bytes;
         const uint8_t* scales = smem + area + ((s - s0) * kStepGroups * kWarpRows + g) * 8;
-#pragma unroll 1
-        for (int half = slice; half < 2; half += slices) {         // 128 k
+        const uint8_t* codes = at + (slices == 2 ? slice * p.rows * 128 : 0);
+#pragma unroll
+        for (int piece = 0; piece < 4 / slices; ++piece) {         // 128 k
+          const int quarter = slices == 2 ? slice * 2 + piece : piece;
           float part[kMT][kNT][4];
           uint32_t sub0[kMT][2], sub1[kMT][2];
           float scale[kMT][2];
@@ -310,7 +319,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
               for (int a = 0; a < kMT; ++a)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                  const uint2 v = *reinterpret_cast<const uint2*>(scales + (((half * 4 + q) >> kShift) * kWarpRows + a * 16 + r * 8) * 8);
+                  const uint2 v = *reinterpret_cast<const uint2*>(scales + (((quarter * 4 + q) >> kShift) * kWarpRows + a * 16 + r * 8) * 8);
                   scale[a][r] = __uint_as_float(v.x);
                   sub0[a][r] = v.y;
                   if (!kBf16) sub1[a][r] = H::fma(sub0[a][r], H::kOne, H::kStep);      // -(64 + z)
@@ -319,13 +328,14 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
             uint4 x[kNT];
 #pragma unroll
             for (int b = 0; b < kNT; ++b)
-              x[b] = *reinterpret_cast<const uint4*>(at + (x_first ^ ((q & 1) << 6)) + (half * 2 + (q >> 1)) * (kMp * 128) + b * 1024);
+              x[b] = *reinterpret_cast<const uint4*>(at + (x_first ^ ((q & 1) << 6)) + (quarter * 2 + (q >> 1)) * (kMp * 128) + b * 1024);
 #pragma unroll
             for (int a = 0; a < kMT; ++a) {
               uint32_t w[2][4];
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const uint32_t lo = *reinterpret_cast<const uint32_t*>(at + (w_first ^ (q << 4) ^ (half << 6)) + a * 2048 + r * 1024);
+                const uint32_t lo = *reinterpret_cast<const uint32_t*>(codes + (w_first ^ (q << 4) ^ ((piece & 1) << 6)) +
+                                                                      (slices == 1 ? (piece >> 1) * p.rows * 128 : 0) + a * 2048 + r * 1024);
                 const uint32_t hi = lo >> 8;
                 w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
                 w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
@@ -422,19 +432,19 @@ struct Plan {
 template <typename Resident>
 Plan w4_plan(int64_t n, int64_t k, int nt, Resident resident) {
   const int64_t steps = (k + kStageK - 1) / kStageK;
-  const int step = 16 * tiles(nt), most = step * consumers(nt) < kMaxRows ? step * consumers(nt) : kMaxRows;
+  const int step = 16 * tiles(nt), most = step * consumers(nt) < max_rows(nt) ? step * consumers(nt) : max_rows(nt);
   Plan best = {step, 1};
   int64_t best_cost = INT64_MAX;
   for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2) {
-    if (cluster > (steps + 1) / 2) break;
+    if (cluster > steps) break;
     const int64_t together = resident(cluster);
     if (together <= 0) continue;
     for (int rows = step; rows <= most; rows += step) {
       const int64_t waves = ((n + rows - 1) / rows + together - 1) / together;
       const int units = rows / step, warps = 2 * units <= consumers(nt) ? 2 * units : units;
       const int64_t rate = warps * 20 < 440 ? warps * 20 : 440;    // 0.1 KB per us
-      const int64_t each = ((steps + 1) / 2 + cluster - 1) / cluster * 2;
-      const int64_t cost = waves * (rows * each * 125 / rate + 150 + (cluster > 1 ? 120 : 0));
+      const int64_t each = (steps + cluster - 1) / cluster;
+      const int64_t cost = waves * (rows * each * 250 / rate + 150 + (cluster > 1 ? 120 : 0));
       if (cost < best_cost) { best_cost = cost; best = {rows, cluster}; }
     }
   }
@@ -447,11 +457,12 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   constexpr int smem = 1024 + kRing + consumers(kNT) * warp_area(kNT, kShift) + static_cast<int>(sizeof(W4Tail));
   constexpr int kLaneGroups = super_steps(kNT, kShift) * step_groups(kShift) * tiles(kNT) / 2;
   static_assert(smem <= 227 * 1024, "shared memory of one SM");
-  static_assert(kLaneGroups == 4 || kLaneGroups == 8, "what RawScales loads at once");
-  static_assert(kRing / stage_size(kMaxRows, kNT * 8) >= 2, "two stages at least");
-  auto kernel = w4_kernel<kBf16, kNT, kShift>;
-  static DeviceFlags done;
-  int rc = ensure_smem_limit(kernel, smem, done);
+  static_assert(kLaneGroups == 4 || kLaneGroups % 8 == 0, "what RawScales loads at once");
+  static_assert(kRing / stage_size(max_rows(kNT), kNT * 8) >= 2, "two stages at least");
+  auto whole = w4_kernel<kBf16, kNT, kShift, 1>, halves = w4_kernel<kBf16, kNT, kShift, 2>;
+  static DeviceFlags done_whole, done_halves;
+  int rc = ensure_smem_limit(whole, smem, done_whole);
+  if (rc == BFP8_OK) rc = ensure_smem_limit(halves, smem, done_halves);
   if (rc != BFP8_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads, 1, 1);
@@ -472,12 +483,12 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
     ask.gridDim = dim3(static_cast<unsigned>(cluster), 1, 1);
     ask.attrs = attr + 1;
     ask.numAttrs = 1;
-    return max_active_clusters(kernel, ask, cluster, caps);
+    return max_active_clusters(whole, ask, cluster, caps);
   });
   p.rows = plan.rows;
   p.cluster = plan.cluster;
   p.scale_vec = p.groups % kLaneGroups == 0 && aligned(p.scales, 2 * kLaneGroups) && (p.zeros == nullptr || aligned(p.zeros, kLaneGroups));
-  p.slices = p.rows / (16 * tiles(kNT)) * 2 <= consumers(kNT) ? 2 : 1;
+  const bool two = p.rows / (16 * tiles(kNT)) * 2 <= consumers(kNT);
   const int most = kRing / stage_size(p.rows, kNT * 8);
   p.stages = most < kMaxStages ? most : kMaxStages;
   alignas(64) CUtensorMap tmap_w, tmap_x;
@@ -489,7 +500,7 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>((p.m + kNT * 8 - 1) / (kNT * 8)), 1);
   attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
-  BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmap_w, tmap_x, p));
+  BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, two ? halves : whole, tmap_w, tmap_x, p));
   return BFP8_OK;
 }
 
