@@ -59,6 +59,11 @@ def _row_stride(t, rows, width):
     return t.stride(0) if rows > 1 else width
 
 
+def _rows_apart(t, rows, width):
+    """t itself, or a copy where its rows overlap (a broadcast one): the kernels take any pitch from the width on."""
+    return t.contiguous() if rows > 1 and t.stride(0) < width else t
+
+
 def route_topk(x, router_weight, top_k, *, scoring="softmax", renormalize=True, bias=None, scale=1.0):
     """(ids int32 [T, top_k], weights fp32 [T, top_k]): the experts of every token, in descending order of their score.
 
@@ -73,6 +78,7 @@ def route_topk(x, router_weight, top_k, *, scoring="softmax", renormalize=True, 
     experts = _check_router(dev, h, router_weight, top_k, scoring, bias)
     lib = _lib.load()
     with _device_guard(dev):
+        x, router_weight = _rows_apart(x, t, h), _rows_apart(router_weight, experts, h)
         ids = _empty(t, top_k, _I32, dev)
         weights = _empty(t, top_k, _F32, dev)
         if t == 0:
@@ -128,13 +134,13 @@ def moe_block_fp8(x, ids, weights, w_gate_up, s_gate_up, w_down, s_down, *, nati
                   status=None, max_ctas=0, wait_limit_cycles=0):
     """bf16 [T, H]: out[t] = sum_j weights[t, j] * expert ids[t, j] of x[t], expert e of v = down(silu(gate(v)) * up(v)).
 
-    x          bf16 [T, H], T <= 128;  ids int32 [T, k];  weights fp32 [T, k]
+    x          bf16 [T, H], T <= 128, rows of unit stride;  ids int32 [T, k];  weights fp32 [T, k]
     w_gate_up  E4M3 [E, 2, I, H] (gate, then up), s_gate_up fp32 [E, 2, ceil(I/128), ceil(H/128)]
     w_down     E4M3 [E, H, I],                    s_down    fp32 [E, ceil(H/128), ceil(I/128)]
     H and I are multiples of 16.  x, and silu(gate) * up in fp32, are quantized as quantize_act_1x128(native_half) does.
     A negative id adds nothing (an expert that another GPU holds); one beyond the last expert adds nothing either and,
     with `check`, raises ValueError.  An expert may occur several times in a token.  check, status, max_ctas and
-    wait_limit_cycles as in gemm_block_fp8.  Calls need no workspace of the caller's and may overlap.
+    wait_limit_cycles as in gemm_block_fp8.  Calls need no workspace of the caller's and may overlap; out may be x.
     """
     _check_rows(x)
     t, h = x.shape
@@ -151,6 +157,7 @@ def moe_block_fp8(x, ids, weights, w_gate_up, s_gate_up, w_down, s_down, *, nati
     experts, inter = _check_experts(dev, t, h, k, w_gate_up, s_gate_up, w_down, s_down, out)
     lib = _lib.load()
     with _device_guard(dev):
+        x = _rows_apart(x, t, h)
         if out is None:
             out = _empty(t, h, _BF16, dev)
         if t == 0:
@@ -181,6 +188,7 @@ def moe_layer_block_fp8(x, router_weight, top_k, w_gate_up, s_gate_up, w_down, s
         raise ValueError("router_weight [E, H] and w_gate_up [E, 2, I, H] must share E")
     lib = _lib.load()
     with _device_guard(dev):
+        x, router_weight = _rows_apart(x, t, h), _rows_apart(router_weight, experts, h)
         if out is None:
             out = _empty(t, h, _BF16, dev)
         ids = _empty(t, top_k, _I32, dev)

@@ -52,7 +52,7 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
     x      bf16 or fp16 [M, K], K a multiple of 32; any M, made for up to 32 rows (the weight is read once per 32)
     codes  uint8 [N, K / 2], q of even k in the low four bits;  scales of x's type [N, ceil(K / group)]
     zeros  uint8 of scales' shape, 0 .. 15, or None: 8;  bias fp32 [N] or None;  group 32, 64 or 128
-    out    of x's type, or float32 with out_dtype=torch.float32
+    out    of x's type, or float32 with out_dtype=torch.float32; may not overlap x
     check  read the status word after the launch (one synchronisation) and raise if a bounded wait expired; status as in
            gemm_block_fp8.  The kernel waits for nothing but its own copies, so calls are unchecked by default.
     """
@@ -92,8 +92,8 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
             out = _empty(m, n, out_dtype, dev)
         if m == 0:
             return out
-        if x.data_ptr() % 16 or (m > 1 and x.stride(0) % 8):
-            x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries
+        if x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
+            x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries, each its own
         st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
         rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, kind, codes.data_ptr(),
                                     scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,

@@ -161,6 +161,45 @@ def test_strided_rows_and_a_given_output(gk):
     assert (big[0] == 3).all() and (big[6] == 3).all() and (big[:, :4] == 3).all() and (big[:, 276:] == 3).all()
 
 
+def test_broadcast_rows_and_an_output_in_place(gk):
+    x, ids, weights, *w = [a.to(DEV) for a in _problem(6, 2, 4, 272, 128)]
+    same = x[2:3].expand(6, 272)
+    want = gk.moe_block_fp8(same.contiguous(), ids, weights, *w)
+    assert torch.equal(gk.moe_block_fp8(same, ids, weights, *w), want)
+    r = torch.randn((4, 272), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    for a, b in zip(gk.route_topk(same, r, 2), gk.route_topk(same.contiguous(), r, 2)):
+        assert torch.equal(a, b)
+    want, keep = gk.moe_block_fp8(x, ids, weights, *w), x.clone()
+    assert gk.moe_block_fp8(x, ids, weights, *w, out=x) is x and torch.equal(x, want)
+    x.copy_(keep)
+    want = gk.moe_layer_block_fp8(x, r, 2, *w)
+    got = gk.moe_layer_block_fp8(x, r, 2, *w, out=x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_many_calls_of_several_shapes_at_once(gk):
+    # cooperative launches of four streams beside a library product: every wait ends, every result is the lone call's
+    from gaudi_kernels_b200.block_fp8_gemm import new_status
+    shapes = ((1, 8, 32, 512, 384), (12, 4, 16, 1040, 656), (40, 4, 32, 512, 256), (128, 8, 32, 256, 128))
+    args = [[a.to(DEV) for a in _problem(*s)] for s in shapes]
+    want = [gk.moe_block_fp8(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in range(5)]
+    status = [new_status(torch.device(DEV)) for _ in args]
+    big = torch.ones((4096, 4096), dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    outs = [[] for _ in args]
+    for n in range(40):
+        for i, a in enumerate(args):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(gk.moe_block_fp8(*a, check=False, status=status[i]))
+        if n % 8 == 0:
+            with torch.cuda.stream(streams[4]):
+                big @ big
+    torch.cuda.synchronize()
+    assert all(s.tolist()[2] == 0 for s in status)
+    assert all(torch.equal(o, w) for got, w in zip(outs, want) for o in got)
+
+
 def test_results_repeat_and_calls_overlap(gk):
     args = [a.to(DEV) for a in _problem(12, 4, 8, 640, 400)]
     want = gk.moe_block_fp8(*args)

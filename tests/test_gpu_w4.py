@@ -99,6 +99,13 @@ def test_strided_rows_and_a_given_output(gk):
     assert (big[0] == 3).all() and (big[6] == 3).all() and (big[:, :7] == 3).all() and (big[:, 137:] == 3).all()
 
 
+def test_broadcast_rows(gk):
+    x, codes, scales, z = _problem(5, 130, 256, 64, torch.bfloat16, True)
+    same = _dev(x)[2:3].expand(5, 256)
+    want = gk.gemm_group_w4(same.contiguous(), _dev(codes), _dev(scales), _dev(z), group=64)
+    assert torch.equal(gk.gemm_group_w4(same, _dev(codes), _dev(scales), _dev(z), group=64), want)
+
+
 def test_nonfinite_rows_stay_alone(gk):
     x, codes, scales, z = _problem(6, 200, 512, 128, torch.bfloat16, True)
     x[2, 17], x[4, 300] = float("nan"), float("inf")
