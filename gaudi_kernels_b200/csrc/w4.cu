@@ -10,11 +10,16 @@
 //     need the unpacked operand in shared memory, four times the bytes that come from HBM.
 //   * which k a thread's operand register stands for is free as long as A and B agree: a thread owns 8 consecutive k of each
 //     32, the word as it lies in memory, and pairs (k, k + 4) of x by byte permutes.
-//   * the weight streams through a ring of shared-memory stages, 256 k of the CTA's rows each, by TMA; x comes with it.
-//     Scales and zero points go from global memory to registers one stage ahead and are handed round by shuffles.
+//   * the weight streams through a ring of shared-memory stages, 512 k of the CTA's rows each, by TMA; x comes with it, and one
+//     warp per 8 activation rows makes the permutes once for all others.  Scales and zero points go from global memory to
+//     the registers of the warp that has their rows, up to 1024 k ahead, and from there to its shared memory as fp32 scale
+//     and 16-bit offset.
 //   * a CTA has R rows (a multiple of 16) and a slice of K: R and the cluster size are chosen so that the CTAs fill the SMs
-//     once with the least per CTA (w4_plan).  Inside the CTA the warps split R and, where that leaves warps over, the
-//     stages; the CTAs of a cluster add their sums through distributed shared memory.  All sums in a fixed order.
+//     once with the least per CTA (w4_plan).  Inside the CTA the warps split R and, where that leaves warps over, the k of
+//     a stage; the CTAs of a cluster add their sums through distributed shared memory.  All sums in a fixed order.
+// Measured: 10.2 us for 1 x 14336 x 4096 (2.9 TB/s), 32 us for 8 x 28672 x 8192 with groups of 64 (4.0 TB/s).  The copies alone
+// take 7 and 19.6 us, the multiplication alone of resident data 9 and 28: what is left bounds it is unpacking, 8 LOP3, 8
+// HFMA2 and 2 to 6 shifts per 512 weights and warp, in chains that three or four warps per scheduler do not hide.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -113,21 +118,16 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-// kNT: activation rows / 8; kMT: 16-row weight tiles per warp (x is read from shared memory once for all of them);
-// kShift: group = 32 << kShift.
 // Warps that multiply, warps that rearrange x (one per 8 activation rows), and one that copies
 __host__ __device__ constexpr int consumers(int nt) { return 15 - nt; }
 constexpr int kThreads = 16 * 32;
-// 16-row weight tiles per warp: with many activation rows two, so that x is read from shared memory once for both
-__host__ __device__ constexpr int tiles(int nt) { return nt >= 4 ? 2 : 1; }
 // Scales are fetched for up to 1024 k at once: from the [n, groups] layout 256 k of a row are 4 to 16 bytes of a 128-byte line,
 // and a warp-wide load costs a cycle per line
-__host__ __device__ constexpr int super_steps(int nt, int shift) { return shift == 0 || tiles(nt) == 2 ? 1 : 2; }
+__host__ __device__ constexpr int super_steps(int shift) { return shift == 0 ? 1 : 2; }
 __host__ __device__ constexpr int step_groups(int shift) { return kStageK >> (5 + shift); }
-__host__ __device__ constexpr int warp_area(int nt, int shift) { return 16 * tiles(nt) * super_steps(nt, shift) * step_groups(shift) * 8; }
-__host__ __device__ constexpr int ring_bytes(int nt, int shift) { return (kSmemBytes - consumers(nt) * warp_area(nt, shift)) & ~1023; }
-// weight rows per CTA: a TMA box at most, and two stages have to fit
-__host__ __device__ constexpr int max_rows(int nt) { return nt >= 4 ? 192 : 256; }
+__host__ __device__ constexpr int warp_area(int shift) { return 16 * super_steps(shift) * step_groups(shift) * 8; }
+__host__ __device__ constexpr int ring_bytes(int nt, int shift) { return (kSmemBytes - consumers(nt) * warp_area(shift)) & ~1023; }
+constexpr int kMaxRows = 256;                              // weight rows per CTA: a TMA box at most
 __host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * (kStageK / 2) + mp * kStageK * 2; }
 
 // Scales and zero points of kGroups neighbouring groups of one row as they lie in memory, loaded well before they are used
@@ -176,15 +176,15 @@ template <bool kBf16, int kNT, int kShift, int kSlices>
 __global__ void __launch_bounds__(kThreads, 1)
 w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Params p) {
   using H = Half16<kBf16>;
-  constexpr int kConsumers = consumers(kNT), kProducer = 15, kMT = tiles(kNT), kWarpRows = 16 * kMT;
+  constexpr int kConsumers = consumers(kNT), kProducer = 15, kWarpRows = 16;
   constexpr int kMp = kNT * 8;
   constexpr int kXBytes = kMp * kStageK * 2;
-  constexpr int kStepGroups = step_groups(kShift), kSuper = super_steps(kNT, kShift);
-  constexpr int kLaneGroups = kSuper * kStepGroups * kMT / 2;      // 4, 8 or 16: two lanes per row with one tile, one with two
+  constexpr int kStepGroups = step_groups(kShift), kSuper = super_steps(kShift);
+  constexpr int kLaneGroups = kSuper * kStepGroups / 2;            // 4 or 8: two lanes per row
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + ring_bytes(kNT, kShift) + kConsumers * warp_area(kNT, kShift));
+  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + ring_bytes(kNT, kShift) + kConsumers * warp_area(kShift));
   volatile uint32_t* abort_flag = &tail->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.rows / kWarpRows;                            // warps across R
@@ -209,13 +209,11 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   __syncthreads();
   ptx::griddep_launch_dependents();
 
-  float acc[kMT][kNT][4];
+  float acc[kNT][4];
 #pragma unroll
-  for (int a = 0; a < kMT; ++a)
+  for (int b = 0; b < kNT; ++b)
 #pragma unroll
-    for (int b = 0; b < kNT; ++b)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[a][b][c] = 0.0f;
+    for (int c = 0; c < 4; ++c) acc[b][c] = 0.0f;
   const int unit = warp % units, slice = warp / units;
   const int g = lane >> 2, t = lane & 3;
   // activation row of column g of the B operand: neighbouring columns lie in different halves of the swizzled 128 bytes
@@ -278,10 +276,10 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     }
   } else if (slice < slices) {
     // ------------------------------------------------------------------ consumers
-    const uint32_t area = ring_bytes(kNT, kShift) + warp * warp_area(kNT, kShift);
-    // this lane's share of the scales: a row, and with one tile per warp one half of the groups
-    const int row = kMT == 1 ? lane & 15 : lane, share = kMT == 1 ? (lane >> 4) * kLaneGroups : 0;
-    const uint32_t w_first = unit * kMT * 2048 + g * 128 + (g << 4) + t * 4;      // chunk c of 16 bytes of row r lies at c ^ (r & 7)
+    const uint32_t area = ring_bytes(kNT, kShift) + warp * warp_area(kShift);
+    // this lane's share of the scales: one half of a row's groups
+    const int row = lane & 15, share = (lane >> 4) * kLaneGroups;
+    const uint32_t w_first = unit * 2048 + g * 128 + (g << 4) + t * 4;      // chunk c of 16 bytes of row r lies at c ^ (r & 7)
     const uint32_t x_first = p.rows * 256 + xrow * 128 + ((t ^ xrow) << 4);
     ptx::griddep_wait();
     RawScales<kLaneGroups> raw;
@@ -308,57 +306,51 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 #pragma unroll
         for (int piece = 0; piece < 4 / slices; ++piece) {         // 128 k
           const int quarter = slices == 2 ? slice * 2 + piece : piece;
-          float part[kMT][kNT][4];
-          uint32_t sub0[kMT][2], sub1[kMT][2];
-          float scale[kMT][2];
+          float part[kNT][4], scale[2];
+          uint32_t sub0[2], sub1[2];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             constexpr int kMask = (1 << kShift) - 1;
             if ((q & kMask) == 0) {                                // a new group
 #pragma unroll
-              for (int a = 0; a < kMT; ++a)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                  const uint2 v = *reinterpret_cast<const uint2*>(scales + (((quarter * 4 + q) >> kShift) * kWarpRows + a * 16 + r * 8) * 8);
-                  scale[a][r] = __uint_as_float(v.x);
-                  sub0[a][r] = v.y;
-                  if (!kBf16) sub1[a][r] = H::fma(sub0[a][r], H::kOne, H::kStep);      // -(64 + z)
-                }
+              for (int r = 0; r < 2; ++r) {
+                const uint2 v = *reinterpret_cast<const uint2*>(scales + (((quarter * 4 + q) >> kShift) * kWarpRows + r * 8) * 8);
+                scale[r] = __uint_as_float(v.x);
+                sub0[r] = v.y;
+                if (!kBf16) sub1[r] = H::fma(sub0[r], H::kOne, H::kStep);        // -(64 + z)
+              }
             }
             uint4 x[kNT];
 #pragma unroll
             for (int b = 0; b < kNT; ++b)
               x[b] = *reinterpret_cast<const uint4*>(at + (x_first ^ ((q & 1) << 6)) + (quarter * 2 + (q >> 1)) * (kMp * 128) + b * 1024);
+            uint32_t w[2][4];
 #pragma unroll
-            for (int a = 0; a < kMT; ++a) {
-              uint32_t w[2][4];
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const uint32_t lo = *reinterpret_cast<const uint32_t*>(codes + (w_first ^ (q << 4) ^ ((piece & 1) << 6)) +
-                                                                      (slices == 1 ? (piece >> 1) * p.rows * 128 : 0) + a * 2048 + r * 1024);
-                const uint32_t hi = lo >> 8;
-                w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-                w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-                if (kBf16) {                                       // seven bits of fraction: no room for a value shifted by four
-                  w[r][1] = H::fma(pick(lo >> 4, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-                  w[r][3] = H::fma(pick(lo >> 12, 0x000f000fu, H::kMagic), H::kOne, sub0[a][r]);
-                } else {                                           // 1024 + 16 q, times 1/16
-                  w[r][1] = H::fma(pick(lo, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
-                  w[r][3] = H::fma(pick(hi, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[a][r]);
-                }
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t lo = *reinterpret_cast<const uint32_t*>(codes + (w_first ^ (q << 4) ^ ((piece & 1) << 6)) +
+                                                                     (slices == 1 ? (piece >> 1) * p.rows * 128 : 0) + r * 1024);
+              const uint32_t hi = lo >> 8;
+              w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+              w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+              if (kBf16) {                                         // seven bits of fraction: no room for a value shifted by four
+                w[r][1] = H::fma(pick(lo >> 4, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+                w[r][3] = H::fma(pick(lo >> 12, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+              } else {                                             // 1024 + 16 q, times 1/16
+                w[r][1] = H::fma(pick(lo, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[r]);
+                w[r][3] = H::fma(pick(hi, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[r]);
               }
-#pragma unroll
-              for (int b = 0; b < kNT; ++b) {
-                if ((q & kMask) == 0) H::mma0(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
-                else H::mma(part[a][b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
-                H::mma(part[a][b], w[0][2], w[1][2], w[0][3], w[1][3], x[b].z, x[b].w);
-              }
-              if ((q & kMask) == kMask)
-#pragma unroll
-                for (int b = 0; b < kNT; ++b)
-#pragma unroll
-                  for (int c = 0; c < 4; ++c) acc[a][b][c] = fmaf(part[a][b][c], scale[a][c >> 1], acc[a][b][c]);
             }
+#pragma unroll
+            for (int b = 0; b < kNT; ++b) {
+              if ((q & kMask) == 0) H::mma0(part[b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
+              else H::mma(part[b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
+              H::mma(part[b], w[0][2], w[1][2], w[0][3], w[1][3], x[b].z, x[b].w);
+            }
+            if ((q & kMask) == kMask)
+#pragma unroll
+              for (int b = 0; b < kNT; ++b)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[b][c] = fmaf(part[b][c], scale[c >> 1], acc[b][c]);
           }
         }
         __syncwarp();
@@ -375,12 +367,10 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   const int width = p.rows;
   if (warp < kConsumers && slice < slices) {
 #pragma unroll
-    for (int a = 0; a < kMT; ++a)
+    for (int b = 0; b < kNT; ++b)
 #pragma unroll
-      for (int b = 0; b < kNT; ++b)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          red[(slice * kMp + b * 8 + t + 4 * (c & 1)) * width + (unit * kMT + a) * 16 + g + 8 * (c >> 1)] = acc[a][b][c];
+      for (int c = 0; c < 4; ++c)
+        red[(slice * kMp + b * 8 + t + 4 * (c & 1)) * width + unit * 16 + g + 8 * (c >> 1)] = acc[b][c];
   }
   __syncthreads();
   const bool whole = *abort_flag == 0;
@@ -421,31 +411,32 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   if (threadIdx.x == 0 && tail->abort_flag != 0) atomicOr(p.status, BFP8_STATUS_WAIT_TIMEOUT);
 }
 
-// Rows per CTA and CTAs per cluster: the least time for the CTA that has most to do.  Measured on B200, in 0.01 us: a warp
-// gets through 2 KB of codes per us, a CTA through its share of the HBM rate (44 KB per us) at most, a wave of CTAs takes
-// 1.5 us to start and a cluster 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with clusters of four,
-// 7.2 us without; 1 row x 1024 x 1024: 3.0 us without, 4.4 us with pairs).  resident(c): clusters of c CTAs that the device
-// holds at once, fewer than its SMs / c where an SM's neighbours are not whole clusters.
+// Rows per CTA and CTAs per cluster: the least time for the CTA that has most to do, priced with what B200 measured, in 0.01 us.
+// The SM's four schedulers have a quarter of the warps each, and the one with most of them sets the pace: one warp unpacks
+// 3.5 KB of codes per us, two 6.6, three 8.5 and four 10 (with 16 activation rows 3, 5.3, 6.5 and 7.5).  A stage costs 0.15 us beside
+// that, a wave of CTAs 1.5 us to start and a cluster 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with
+// clusters of four, 7.2 us without; 1 row x 1024 x 1024: 3.0 us without, 4.4 us with pairs).  resident(c): clusters of c CTAs
+// that the device holds at once - 74 of two, but 33 of four and 15 of eight on 148 SMs.
 struct Plan {
   int rows, cluster;
 };
 template <typename Resident>
-Plan w4_plan(int64_t n, int64_t k, int nt, Resident resident) {
+Plan w4_plan(int64_t n, int64_t k, int64_t chunks, int nt, Resident resident) {
   const int64_t steps = (k + kStageK - 1) / kStageK;
-  const int step = 16 * tiles(nt), most = step * consumers(nt) < max_rows(nt) ? step * consumers(nt) : max_rows(nt);
-  Plan best = {step, 1};
+  const int most = 16 * consumers(nt) < kMaxRows ? 16 * consumers(nt) : kMaxRows;
+  Plan best = {16, 1};
+  constexpr int64_t kRate[2][4] = {{35, 66, 85, 100}, {30, 53, 65, 75}};         // bytes per 0.01 us
   int64_t best_cost = INT64_MAX;
   for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2) {
     if (cluster > steps) break;
     const int64_t together = resident(cluster);
     if (together <= 0) continue;
-    for (int rows = step; rows <= most; rows += step) {
-      const int64_t waves = ((n + rows - 1) / rows + together - 1) / together;
-      const int units = rows / step, warps = 2 * units <= consumers(nt) ? 2 * units : units;
-      const int64_t rate = warps * 20 < 440 ? warps * 20 : 440;    // 0.1 KB per us
-      const int64_t each = (steps + cluster - 1) / cluster;
-      const int64_t cost = waves * (rows * each * 250 / rate + 150 + (cluster > 1 ? 120 : 0));
-      if (cost < best_cost) { best_cost = cost; best = {rows, cluster}; }
+    for (int rows = 16; rows <= most; rows += 16) {
+      const int64_t waves = ((n + rows - 1) / rows * chunks + together - 1) / together;
+      const int units = rows / 16, warps = 2 * units <= consumers(nt) ? 2 * units : units, most_warps = (warps + 3) / 4;
+      const int64_t each = (steps + cluster - 1) / cluster, codes = rows * each * 256 / warps * most_warps;
+      const int64_t cost = waves * (codes / kRate[nt - 1][most_warps - 1] + each * 15 + 150 + (cluster > 1 ? 120 : 0));
+      if (cost < best_cost || (cost == best_cost && cluster > best.cluster)) { best_cost = cost; best = {rows, cluster}; }
     }
   }
   return best;
@@ -454,11 +445,11 @@ Plan w4_plan(int64_t n, int64_t k, int nt, Resident resident) {
 template <bool kBf16, int kNT, int kShift>
 int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
   constexpr int kRing = ring_bytes(kNT, kShift);
-  constexpr int smem = 1024 + kRing + consumers(kNT) * warp_area(kNT, kShift) + static_cast<int>(sizeof(W4Tail));
-  constexpr int kLaneGroups = super_steps(kNT, kShift) * step_groups(kShift) * tiles(kNT) / 2;
+  constexpr int smem = 1024 + kRing + consumers(kNT) * warp_area(kShift) + static_cast<int>(sizeof(W4Tail));
+  constexpr int kLaneGroups = super_steps(kShift) * step_groups(kShift) / 2;
   static_assert(smem <= 227 * 1024, "shared memory of one SM");
-  static_assert(kLaneGroups == 4 || kLaneGroups % 8 == 0, "what RawScales loads at once");
-  static_assert(kRing / stage_size(max_rows(kNT), kNT * 8) >= 2, "two stages at least");
+  static_assert(kLaneGroups == 4 || kLaneGroups == 8, "what RawScales loads at once");
+  static_assert(kRing / stage_size(kMaxRows, kNT * 8) >= 2, "two stages at least");
   auto whole = w4_kernel<kBf16, kNT, kShift, 1>, halves = w4_kernel<kBf16, kNT, kShift, 2>;
   static DeviceFlags done_whole, done_halves;
   int rc = ensure_smem_limit(whole, smem, done_whole);
@@ -476,7 +467,8 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   static ClusterCaps caps;
-  const Plan plan = w4_plan(p.n, p.k, kNT, [&](int cluster) -> int {
+  const int64_t chunks = (p.m + kNT * 8 - 1) / (kNT * 8);
+  const Plan plan = w4_plan(p.n, p.k, chunks, kNT, [&](int cluster) -> int {
     if (cluster == 1) return sm_count();
     cudaLaunchConfig_t ask = cfg;
     attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
@@ -488,7 +480,7 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   p.rows = plan.rows;
   p.cluster = plan.cluster;
   p.scale_vec = p.groups % kLaneGroups == 0 && aligned(p.scales, 2 * kLaneGroups) && (p.zeros == nullptr || aligned(p.zeros, kLaneGroups));
-  const bool two = p.rows / (16 * tiles(kNT)) * 2 <= consumers(kNT);
+  const bool two = p.rows / 16 * 2 <= consumers(kNT);
   const int most = kRing / stage_size(p.rows, kNT * 8);
   p.stages = most < kMaxStages ? most : kMaxStages;
   alignas(64) CUtensorMap tmap_w, tmap_x;
@@ -497,7 +489,7 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   rc = make_tensor_map_2d(&tmap_x, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, p.k, p.m,
                           ldx * 2, 64, kNT * 8);
   if (rc != BFP8_OK) return rc;
-  cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>((p.m + kNT * 8 - 1) / (kNT * 8)), 1);
+  cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>(chunks), 1);
   attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
   BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, two ? halves : whole, tmap_w, tmap_x, p));
@@ -513,9 +505,10 @@ int launch_group(int group, const uint8_t* codes, const void* x, int64_t ldx, W4
 
 template <bool kBf16>
 int launch_rows(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  if (p.m <= 8) return launch_group<kBf16, 1>(group, codes, x, ldx, p, st);
-  if (p.m <= 16) return launch_group<kBf16, 2>(group, codes, x, ldx, p, st);
-  return launch_group<kBf16, 4>(group, codes, x, ldx, p, st);
+  // More than 16 rows in several passes over the weight: with the sums of 32 rows in its registers a warp spilled, and took
+  // 22.9 us for 32 x 4096 x 14336, 28.5 for 32 x 14336 x 4096 and 92 for 32 x 28672 x 8192 where two passes of 16 rows take
+  // 23.2, 24.1 and 77.
+  return p.m <= 8 ? launch_group<kBf16, 1>(group, codes, x, ldx, p, st) : launch_group<kBf16, 2>(group, codes, x, ldx, p, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
