@@ -177,6 +177,15 @@ def test_broadcast_rows_and_an_output_in_place(gk):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_weights_prepared_in_the_half_range(gk):
+    x, ids, weights, w13, s13, w2, s2 = _problem(6, 2, 4, 272, 144)
+    p13, q13 = gk.prepare_weight(w13.view(torch.float8_e4m3fn).to(DEV), s13.to(DEV))
+    p2, q2 = gk.prepare_weight(w2.view(torch.float8_e4m3fn).to(DEV), s2.to(DEV))
+    assert p13.shape == w13.shape and torch.equal(q13.cpu(), 2 * s13)
+    got = gk.moe_block_fp8(x.to(DEV), ids.to(DEV), weights.to(DEV), p13, q13, p2, q2, native_half=True)
+    _check(got, (x, ids, weights, p13.cpu().view(torch.uint8), q13.cpu(), p2.cpu().view(torch.uint8), q2.cpu()), True)
+
+
 def test_many_calls_of_several_shapes_at_once(gk):
     # cooperative launches of four streams beside a library product: every wait ends, every result is the lone call's
     from gaudi_kernels_b200.block_fp8_gemm import new_status
