@@ -650,6 +650,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
           if (lane == 0) there = wait_word(p.sync + kSyncChunks + c.chunk, p.gi, abort_flag, p.wait_limit);
           ok = __all_sync(0xffffffffu, there);
           if (!ok) break;
+          __syncwarp();                                            // a vote alone orders no memory
           fence_proxy_async();                                     // h was written by ordinary stores, TMA reads it
           seen = c.chunk;
         }
@@ -719,6 +720,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
           bool there = true;
           if (lane == 0) there = wait_word(p.sync + kSyncChunks + f.chunk, p.gi, abort_flag, p.wait_limit);
           ok = ok && __all_sync(0xffffffffu, there);
+          __syncwarp();
           seen = f.chunk;
         }
         if (phase == 0) {
@@ -1075,6 +1077,7 @@ int moe_layer(const uint16_t* x, int64_t ldx, const Router* router, const int32_
               size_t workspace_bytes, uint32_t* status_dev, void* stream, int max_ctas, int64_t wait_limit_cycles) {
   if (!x || !w13 || !s13 || !w2 || !s2 || !out || !status_dev || !workspace) return BFP8_ERR_NULL;
   if (router ? !router->weight : (!ids || !weights)) return BFP8_ERR_NULL;
+  if (!router && (!aligned(ids, 4) || !aligned(weights, 4))) return BFP8_ERR_ALIGN;
   if (t <= 0 || k <= 0 || e <= 0 || h <= 0 || i <= 0 || h > kMaxWidth || i > kMaxWidth || ldx < h || ldo < h) return BFP8_ERR_SHAPE;
   if (t > kMaxTokens || k > kMaxTopK || e > kMaxExperts || t * k > kMaxSlots || h % 16 != 0 || i % 16 != 0)
     return BFP8_ERR_UNSUPPORTED;

@@ -143,3 +143,7 @@ def test_strides_and_arguments_of_the_calls(lib):          # noqa: F811
     args = lib.named("bfp8_moe_block128")[0]
     assert args[1] == 256 and args[9] == 256               # one row: the stride is free, the width is given
     assert args[10:16] == (1, 2, 8, 256, 144, 1) and args[20] == 3
+
+
+def test_misaligned_choices(so):
+    assert _experts(so, ids=A + 2) == -2 and _experts(so, weights=A + 1) == -2
