@@ -127,6 +127,7 @@ __host__ __device__ constexpr int super_steps(int shift) { return shift == 0 ? 1
 __host__ __device__ constexpr int step_groups(int shift) { return kStageK >> (5 + shift); }
 __host__ __device__ constexpr int warp_area(int shift) { return 16 * super_steps(shift) * step_groups(shift) * 8; }
 __host__ __device__ constexpr int ring_bytes(int nt, int shift) { return (kSmemBytes - consumers(nt) * warp_area(shift)) & ~1023; }
+constexpr int64_t kMaxM = 65535 * 16;                      // activation rows: chunks of 16 on the grid's y axis
 constexpr int kMaxRows = 256;                              // weight rows per CTA: a TMA box at most
 __host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * (kStageK / 2) + mp * kStageK * 2; }
 
@@ -270,6 +271,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
               make_uint4(__byte_perm(v[q].x, v[q].z, 0x5410), __byte_perm(v[q].x, v[q].z, 0x7632),
                          __byte_perm(v[q].y, v[q].w, 0x5410), __byte_perm(v[q].y, v[q].w, 0x7632));
       }
+      ptx::fence_proxy_async_smem();                               // the stage's next copy may not pass these stores
       __syncwarp();
       ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->ready[stage]), lane);
       advance();
@@ -518,7 +520,8 @@ template <bool kBf16>
 __device__ __forceinline__ float rounded16(float v) { return Half16<kBf16>::value(Half16<kBf16>::round(v)); }
 
 // zeros != NULL: s = rounded((max(max w, 0) - min(min w, 0)) / 15), z = clamp(rne(-min / s), 0, 15); otherwise
-// s = rounded(max|w| / 7), z = 8.  q = clamp(rne(w / s) + z, 0, 15).  A group of zeros gets s = 1.
+// s = rounded(max|w| / 7), z = 8.  q = clamp(rne(w / s) + z, 0, 15).  A group of zeros gets s = 1, one
+// with a NaN s = NaN; where s overflows it is infinite, and the weights read back are not finite.
 template <bool kBf16>
 __global__ void __launch_bounds__(256)
 quant_group_w4_kernel(const float* __restrict__ w, int64_t n, int k, int64_t ldw, int group, int groups,
@@ -530,8 +533,10 @@ quant_group_w4_kernel(const float* __restrict__ w, int64_t n, int k, int64_t ldw
   const int k0 = static_cast<int>(item - row * groups) * group, len = min(group, k - k0);
   const float* src = w + row * ldw + k0;
   float lo = 0.0f, hi = 0.0f;
+  bool nan = false;
   for (int c = lane; c < len; c += 32) {
     const float v = src[c];
+    nan |= v != v;
     lo = fminf(lo, v);
     hi = fmaxf(hi, v);
   }
@@ -542,6 +547,7 @@ quant_group_w4_kernel(const float* __restrict__ w, int64_t n, int k, int64_t ldw
   }
   float s = rounded16<kBf16>(zeros != nullptr ? __fdiv_rn(hi - lo, 15.0f) : __fdiv_rn(fmaxf(hi, -lo), 7.0f));
   if (s == 0.0f) s = 1.0f;
+  if (__any_sync(0xffffffffu, nan)) s = __uint_as_float(0x7fffffffu);
   const int z = zeros != nullptr ? static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.0f), 15.0f)) : 8;
   if (lane == 0) {
     scales[item] = Half16<kBf16>::round(s);
@@ -564,7 +570,7 @@ extern "C" int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const
                                   const uint8_t* zeros, int group, const float* bias, void* out, int out_f32, int64_t ldo,
                                   int64_t m, int64_t n, int64_t k, uint32_t* status_dev, void* stream, int64_t wait_limit_cycles) {
   if (!x || !codes || !scales || !out || !status_dev) return BFP8_ERR_NULL;
-  if (m <= 0 || n <= 0 || k <= 0 || m > (1 << 20) || n > (1 << 30) || k > (1 << 30) || ldx < k || ldo < n) return BFP8_ERR_SHAPE;
+  if (m <= 0 || n <= 0 || k <= 0 || m > kMaxM || n > (1 << 30) || k > (1 << 30) || ldx < k || ldo < n) return BFP8_ERR_SHAPE;
   if (x_dtype != BFP8_W4_BF16 && x_dtype != BFP8_W4_F16) return BFP8_ERR_SHAPE;
   if (group != 32 && group != 64 && group != 128) return BFP8_ERR_UNSUPPORTED;
   if (k % 32 != 0) return BFP8_ERR_UNSUPPORTED;

@@ -384,7 +384,7 @@ int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* rout
  *   bias    fp32 [n] or NULL;  out of x's type, or fp32 with out_f32 != 0, [m, n], row stride ldo
  * group 32, 64 or 128, k a multiple of 32 (BFP8_ERR_UNSUPPORTED otherwise; the last group may be short).  q - z is exact,
  * sums are formed in fp32 in a fixed order, and a group's sum is multiplied by its scale in fp32.  Made for few rows: the
- * weight is read once per 16 of them.  No workspace.  With bfp8_set_weights_at_rest the codes are requested before
+ * weight is read once per 16 of them; m <= 1048560.  A group's sum is formed before its scale is applied.  No workspace.  With bfp8_set_weights_at_rest the codes are requested before
  * the previous kernel of the stream has ended.  status |= WAIT_TIMEOUT if an internal wait gave up.  The reference has no
  * counterpart. */
 #define BFP8_W4_BF16 0
@@ -395,7 +395,9 @@ int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const uint8_t* c
 
 /* fp32 weight [n, k] (row stride ldw) -> the codes, scales and zero points above.  zeros != NULL:
  * s = round16((max(w, 0) - min(w, 0)) / 15), z = clamp(rne(-min / s), 0, 15); zeros == NULL: s = round16(max|w| / 7),
- * z = 8.  q = clamp(rne(w / s) + z, 0, 15); a group of zeros, or one whose s rounds to zero, gets s = 1. */
+ * z = 8.  q = clamp(rne(w / s) + z, 0, 15); a group of zeros, or one whose s rounds to zero, gets s = 1;
+ * one with a NaN gets s = NaN, and one with an infinity, or whose s overflows the scale's type, s = inf: what it reads
+ * back is then not finite. */
 int bfp8_quant_group_w4_f32(const float* w, int64_t n, int64_t k, int64_t ldw, int group, uint8_t* codes,
                             uint16_t* scales, uint8_t* zeros, int scale_dtype, void* stream);
 

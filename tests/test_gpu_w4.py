@@ -183,6 +183,23 @@ def test_quantizer_bits(gk, n, k, group, zeros, scale_dtype):
         assert (a is None and b is None and c is None) or (torch.equal(a.cpu(), b) and torch.equal(c, b))
 
 
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("scale_dtype", [torch.bfloat16, torch.float16])
+def test_quantizer_groups_that_are_not_finite_stay_alone(gk, scale_dtype, zeros):
+    w = torch.randn((4, 128), generator=torch.Generator().manual_seed(1))
+    want = [v if v is None else v.cpu() for v in gk.quantize_group_w4(w.to(DEV), 32, zeros, scale_dtype)]
+    bad = w.clone()
+    bad[0, 5], bad[1, 40], bad[2, 70], bad[3, 127] = float("nan"), float("inf"), float("-inf"), 3e38 if zeros else float("nan")
+    bad[3, 126] = -3e38                                    # with zero points the range itself overflows
+    codes, scales, z = [v if v is None else v.cpu() for v in gk.quantize_group_w4(bad.to(DEV), 32, zeros, scale_dtype)]
+    for r in range(4):                                     # row r's group r
+        assert not torch.isfinite(scales[r, r]) and (torch.isnan(scales[r, r]) == (r == 0 or r == 3 and not zeros))
+        assert not torch.isfinite(w4_ref.weight(codes, scales, z, 32)[r, 32 * r:32 * r + 32]).any()
+        keep = [g for g in range(4) if g != r]
+        assert torch.equal(scales[r, keep], want[1][r, keep]) and (z is None or torch.equal(z[r, keep], want[2][r, keep]))
+        assert torch.equal(codes.view(4, 4, 16)[r, keep], want[0].view(4, 4, 16)[r, keep])
+
+
 def test_quantized_weight_is_near_the_weight(gk):
     w = torch.randn((40, 512), generator=torch.Generator().manual_seed(4)) * 0.05
     codes, scales, z = gk.quantize_group_w4(w.to(DEV), 64)

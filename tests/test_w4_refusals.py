@@ -110,3 +110,8 @@ def test_rows_and_strides_of_the_call(lib):                # noqa: F811
     gk.gemm_group_w4(**ops, out=out)
     args = lib.named("bfp8_gemm_group_w4")[0]
     assert args[1] == 136 and args[2] == 0 and args[6] == 64 and args[9] == 1 and args[10] == 50 and args[11:14] == (3, 40, 128)
+
+
+@pytest.mark.parametrize("m", [65535 * 16 + 1, 1 << 20])
+def test_more_rows_than_the_grid_holds(so, m):
+    assert so.bfp8_gemm_group_w4(A, 64, 0, A, A, None, 64, None, A, 0, 16, m, 16, 64, A, None, 0) == -3
