@@ -16,9 +16,10 @@
 //     and 16-bit offset.
 //   * a CTA has R rows (a multiple of 16) and a slice of K: R and the cluster size are chosen so that the CTAs fill the SMs
 //     once with the least per CTA (w4_plan).  Inside the CTA the warps split R and, where that leaves warps over, the k of
-//     a stage; the CTAs of a cluster add their sums through distributed shared memory.  All sums in a fixed order.
-// Measured: 10.2 us for 1 x 14336 x 4096 (2.9 TB/s), 32 us for 8 x 28672 x 8192 with groups of 64 (4.0 TB/s).  The copies alone
-// take 7 and 19.6 us, the multiplication alone of resident data 9 and 28: what is left bounds it is unpacking, 8 LOP3, 8
+//     a stage, evenly over the SM's schedulers; the CTAs of a cluster add their sums through distributed shared memory.  All sums in a fixed order.
+// Measured: 10.2 us for 1 x 14336 x 4096 (2.9 TB/s), 31 us for 8 x 28672 x 8192 with groups of 64 (4.1 TB/s).  The copies alone
+// take 7 and 19.6 us, the multiplication alone of resident data 9 and (with whole units
+// per warp only) 28: what bounds it is unpacking, 8 LOP3, 8
 // HFMA2 and 2 to 6 shifts per 512 weights and warp, in chains that three or four warps per scheduler do not hide.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -37,6 +38,7 @@ constexpr long long kDefaultWaitLimit = 2000000000LL;      // about a second
 constexpr int kStageK = 512;                               // k per stage: twice 128 bytes of a code row
 constexpr int kMaxStages = 16;
 constexpr int kSmemBytes = 225 * 1024;
+constexpr int kSmemLimit = 227 * 1024;                     // what one SM has for a CTA
 constexpr int kMaxCluster = 8;
 
 struct W4Params {
@@ -47,6 +49,7 @@ struct W4Params {
   int64_t ldo;
   int m, n, k, groups;
   int rows;                    // R
+  uint32_t row_share;          // 2^32 / R, rounded up: i / R = __umulhi(i, row_share) for the few thousand sums of a CTA
   int stages;                  // ring depth
   int cluster;
   int out_f32;
@@ -112,51 +115,71 @@ __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t mag
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
   return r;
 }
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
 
-// Warps that multiply, warps that rearrange x (one per 8 activation rows), and one that copies
-__host__ __device__ constexpr int consumers(int nt) { return 15 - nt; }
-constexpr int kThreads = 16 * 32;
+// An SM's warps run on four schedulers, warp w on number w % 4, and the one with most work sets the pace.  A CTA's groups of 16
+// rows (units) go to whole warps, each a stage's four pieces of 128 k, or two where a pair of warps shares a unit.  Without a
+// rest that is all; with one, only as many units as divide evenly over the schedulers go to whole warps, and of each unit left
+// over four more warps take a piece each (8 x 28672 x 8192, 13 units: 32.4 us without, 31.1 with; 8 x 35520 x 8192, 15 units:
+// 50 us in two waves without, 36 with; 16 x 65536 x 1024: 21.1 and 18.6).  The rest's code costs 0.5 us where nothing is left.
+// (Quarters of a stage for all warps alike, which needs every unit's scales in reach of four warps: 36 us for 28672 x 8192.)
+__host__ __device__ constexpr int whole_warps(int nt, bool rest) { return rest ? 12 : 15 - nt; }
+__host__ __device__ constexpr int consumers(int nt, bool rest) { return whole_warps(nt, rest) + (rest ? 4 : 0); }
+// ... then one warp per 8 rows of x, and the producer
+__host__ __device__ constexpr int threads_of(int nt, bool rest) { return 32 * (consumers(nt, rest) + nt + 1); }
+__host__ __device__ constexpr int whole_units(int units, int slices, bool rest) {
+  return !rest ? units : slices == 2 ? units & ~1 : min(units & ~3, whole_warps(1, true));
+}
 // Scales are fetched for up to 1024 k at once: from the [n, groups] layout 256 k of a row are 4 to 16 bytes of a 128-byte line,
 // and a warp-wide load costs a cycle per line
 __host__ __device__ constexpr int super_steps(int shift) { return shift == 0 ? 1 : 2; }
 __host__ __device__ constexpr int step_groups(int shift) { return kStageK >> (5 + shift); }
 __host__ __device__ constexpr int warp_area(int shift) { return 16 * super_steps(shift) * step_groups(shift) * 8; }
-__host__ __device__ constexpr int ring_bytes(int nt, int shift) { return (kSmemBytes - consumers(nt) * warp_area(shift)) & ~1023; }
+__host__ __device__ constexpr int rest_area(int shift) { return 3 * 16 * (step_groups(shift) / 4) * 8; }
+__host__ __device__ constexpr int scale_bytes(int nt, int shift, bool rest) {
+  return whole_warps(nt, rest) * warp_area(shift) + (rest ? 4 * rest_area(shift) : 0);
+}
+__host__ __device__ constexpr int ring_bytes(int nt, int shift, bool rest) { return (kSmemBytes - scale_bytes(nt, shift, rest)) & ~1023; }
 constexpr int64_t kMaxM = 65535 * 16;                      // activation rows: chunks of 16 on the grid's y axis
-constexpr int kMaxRows = 256;                              // weight rows per CTA: a TMA box at most
+constexpr int kMaxRows = 16 * (whole_warps(1, true) + 3);                // weight rows per CTA, within a TMA box
 __host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * (kStageK / 2) + mp * kStageK * 2; }
 
 // Scales and zero points of kGroups neighbouring groups of one row as they lie in memory, loaded well before they are used
 template <int kGroups>
 struct RawScales {
-  uint32_t s[kGroups / 2];
-  uint32_t z[kGroups / 4];
+  uint32_t s[(kGroups + 1) / 2];
+  uint32_t z[(kGroups + 3) / 4];
   __device__ __forceinline__ void load(const W4Params& p, int row, int g0) {
 #pragma unroll
-    for (int i = 0; i < kGroups / 2; ++i) s[i] = 0u;
+    for (int i = 0; i < (kGroups + 1) / 2; ++i) s[i] = 0u;
 #pragma unroll
-    for (int i = 0; i < kGroups / 4; ++i) z[i] = 0x08080808u;
+    for (int i = 0; i < (kGroups + 3) / 4; ++i) z[i] = 0x08080808u;
     if (row >= p.n || g0 >= p.groups) return;
     const int64_t at = static_cast<int64_t>(row) * p.groups + g0;
     if (p.scale_vec) {                                             // groups % kGroups == 0: they exist together
-      if (kGroups == 4) {
+      if constexpr (kGroups == 1) {
+        s[0] = __ldg(p.scales + at);
+        if (p.zeros != nullptr) z[0] = __ldg(p.zeros + at);
+      } else if constexpr (kGroups == 2) {
+        s[0] = __ldg(reinterpret_cast<const uint32_t*>(p.scales + at));
+        if (p.zeros != nullptr) z[0] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + at));
+      } else if constexpr (kGroups == 4) {
         const uint2 v = __ldg(reinterpret_cast<const uint2*>(p.scales + at));
         s[0] = v.x; s[1] = v.y;
         if (p.zeros != nullptr) z[0] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
       } else {
-#pragma unroll
-        for (int i = 0; i < kGroups / 8; ++i) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.scales + at + 8 * i));
-          s[4 * i] = v.x; s[4 * i + 1] = v.y; s[4 * i + 2 < kGroups / 2 ? 4 * i + 2 : 0] = v.z; s[4 * i + 3 < kGroups / 2 ? 4 * i + 3 : 0] = v.w;
-          if (p.zeros != nullptr) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.zeros + at + 8 * i));
-            z[2 * i] = u.x; z[2 * i + 1 < kGroups / 4 ? 2 * i + 1 : 0] = u.y;
-          }
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.scales + at));
+        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
+        if (p.zeros != nullptr) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.zeros + at));
+          z[0] = u.x; z[1] = u.y;
         }
       }
     } else {
@@ -169,27 +192,37 @@ struct RawScales {
         }
     }
   }
+  // group j as the kernel uses it: fp32 scale, and -(128 + z) or -(1024 + z) twice
+  template <typename H>
+  __device__ __forceinline__ uint2 ready(int j) const {
+    const uint32_t sc = (s[j >> 1] >> (16 * (j & 1))) & 0xffffu, zp = (z[j >> 2] >> (8 * (j & 3))) & 0xffu;
+    return make_uint2(__float_as_uint(H::value(sc)), H::kMinus + zp * 0x10001u);
+  }
 };
 
-// kNT: activation rows / 8; kShift: group = 32 << kShift; kSlices: warps that share a row range, 2 take a half of each
-// stage's k each.
-template <bool kBf16, int kNT, int kShift, int kSlices>
-__global__ void __launch_bounds__(kThreads, 1)
+// kNT: activation rows / 8; kShift: group = 32 << kShift; kSlices: warps that share 16 rows, 2 take a half of each stage's k
+// each; kRest: four more warps for the units left over.
+template <bool kBf16, int kNT, int kShift, int kSlices, bool kRest>
+__global__ void __launch_bounds__(threads_of(kNT, kRest), 1)
 w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Params p) {
   using H = Half16<kBf16>;
-  constexpr int kConsumers = consumers(kNT), kProducer = 15, kWarpRows = 16;
+  constexpr int kWhole = whole_warps(kNT, kRest), kConsumers = consumers(kNT, kRest), kProducer = kConsumers + kNT;
+  constexpr int kWarpRows = 16, kThreads = threads_of(kNT, kRest), kRing = ring_bytes(kNT, kShift, kRest);
   constexpr int kMp = kNT * 8;
   constexpr int kXBytes = kMp * kStageK * 2;
   constexpr int kStepGroups = step_groups(kShift), kSuper = super_steps(kShift);
   constexpr int kLaneGroups = kSuper * kStepGroups / 2;            // 4 or 8: two lanes per row
+  constexpr int kPieceGroups = kStepGroups / 4;                    // 4, 2 or 1
+  constexpr int kRestUnits = kSlices == 2 ? 1 : 3;                 // groups of rows left over, at most
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + ring_bytes(kNT, kShift) + kConsumers * warp_area(kShift));
+  W4Tail* tail = reinterpret_cast<W4Tail*>(smem + kRing + scale_bytes(kNT, kShift, kRest));
   volatile uint32_t* abort_flag = &tail->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = p.rows / kWarpRows;                            // warps across R
-  constexpr int slices = kSlices;                                  // warps across the k of a stage
+  const int units = p.rows / kWarpRows;
+  constexpr int slices = kSlices;
+  const int whole = whole_units(units, slices, kRest), rest = units - whole;
   const uint32_t stage_bytes = static_cast<uint32_t>(stage_size(p.rows, kMp));
   const int rank = p.cluster > 1 ? static_cast<int>(blockIdx.x) % p.cluster : 0;
   const int n0 = static_cast<int>(blockIdx.x) / p.cluster * p.rows;
@@ -202,7 +235,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     for (int s = 0; s < p.stages; ++s) {
       ptx::mbar_init(ptx::smem_u32(&tail->full[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&tail->ready[s]), kNT);
-      ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), static_cast<uint32_t>(units * slices));
+      ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), static_cast<uint32_t>(whole * slices + (rest > 0 ? 4 : 0)));
     }
     tail->abort_flag = 0;
     ptx::fence_mbar_init();
@@ -210,12 +243,6 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   __syncthreads();
   ptx::griddep_launch_dependents();
 
-  float acc[kNT][4];
-#pragma unroll
-  for (int b = 0; b < kNT; ++b)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[b][c] = 0.0f;
-  const int unit = warp % units, slice = warp / units;
   const int g = lane >> 2, t = lane & 3;
   // activation row of column g of the B operand: neighbouring columns lie in different halves of the swizzled 128 bytes
   const int xrow = (g >> 1) + 4 * (g & 1);
@@ -276,117 +303,181 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
       ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->ready[stage]), lane);
       advance();
     }
-  } else if (slice < slices) {
-    // ------------------------------------------------------------------ consumers
-    const uint32_t area = ring_bytes(kNT, kShift) + warp * warp_area(kShift);
-    // this lane's share of the scales: one half of a row's groups
-    const int row = lane & 15, share = (lane >> 4) * kLaneGroups;
-    const uint32_t w_first = unit * 2048 + g * 128 + (g << 4) + t * 4;      // chunk c of 16 bytes of row r lies at c ^ (r & 7)
+  } else {
+    // ------------------------------------------------------------------ multiplying warps
+    const uint32_t w_lane = g * 128 + (g << 4) + t * 4;                    // chunk c of 16 bytes of row r lies at c ^ (r & 7)
     const uint32_t x_first = p.rows * 256 + xrow * 128 + ((t ^ xrow) << 4);
-    ptx::griddep_wait();
-    RawScales<kLaneGroups> raw;
-    raw.load(p, n0 + unit * kWarpRows + row, step0 * kStepGroups + share);
-    for (int s0 = step0; s0 < step1; s0 += kSuper) {
-      __syncwarp();                                                // the last scales have been read
+    // 16 rows x 128 k: `at` the stage, codes those of the rows' 256 k that hold the piece, scales its first group
+    auto multiply = [&](const uint8_t* at, const uint8_t* codes, const uint8_t* scales, int quarter, float (&acc)[kNT][4]) {
+      float part[kNT][4], scale[2];
+      uint32_t sub0[2], sub1[2];
 #pragma unroll
-      for (int j = 0; j < kLaneGroups; ++j) {
-        const uint32_t sc = (raw.s[j >> 1] >> (16 * (j & 1))) & 0xffffu, z = (raw.z[j >> 2] >> (8 * (j & 3))) & 0xffu;
-        *reinterpret_cast<uint2*>(smem + area + ((share + j) * kWarpRows + row) * 8) =
-            make_uint2(__float_as_uint(H::value(sc)), H::kMinus + z * 0x10001u);
-      }
-      __syncwarp();
-      if (s0 + kSuper < step1) raw.load(p, n0 + unit * kWarpRows + row, (s0 + kSuper) * kStepGroups + share);
-      const int s1 = min(s0 + kSuper, step1);
-      bool ok = true;
-      for (int s = s0; s < s1; ++s) {
-        // x is ready: so are the codes, whose copies the x warps waited for
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->ready[stage]), parity, abort_flag, p.wait_limit));
-        if (!ok) break;
-        const uint8_t* at = smem + stage * stage_bytes;
-        const uint8_t* scales = smem + area + ((s - s0) * kStepGroups * kWarpRows + g) * 8;
-        const uint8_t* codes = at + (slices == 2 ? slice * p.rows * 128 : 0);
+      for (int q = 0; q < 4; ++q) {
+        constexpr int kMask = (1 << kShift) - 1;
+        if ((q & kMask) == 0) {                                            // a new group
 #pragma unroll
-        for (int piece = 0; piece < 4 / slices; ++piece) {         // 128 k
-          const int quarter = slices == 2 ? slice * 2 + piece : piece;
-          float part[kNT][4], scale[2];
-          uint32_t sub0[2], sub1[2];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            constexpr int kMask = (1 << kShift) - 1;
-            if ((q & kMask) == 0) {                                // a new group
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const uint2 v = *reinterpret_cast<const uint2*>(scales + (((quarter * 4 + q) >> kShift) * kWarpRows + r * 8) * 8);
-                scale[r] = __uint_as_float(v.x);
-                sub0[r] = v.y;
-                if (!kBf16) sub1[r] = H::fma(sub0[r], H::kOne, H::kStep);        // -(64 + z)
-              }
-            }
-            uint4 x[kNT];
-#pragma unroll
-            for (int b = 0; b < kNT; ++b)
-              x[b] = *reinterpret_cast<const uint4*>(at + (x_first ^ ((q & 1) << 6)) + (quarter * 2 + (q >> 1)) * (kMp * 128) + b * 1024);
-            uint32_t w[2][4];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const uint32_t lo = *reinterpret_cast<const uint32_t*>(codes + (w_first ^ (q << 4) ^ ((piece & 1) << 6)) +
-                                                                     (slices == 1 ? (piece >> 1) * p.rows * 128 : 0) + r * 1024);
-              const uint32_t hi = lo >> 8;
-              w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
-              w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
-              if (kBf16) {                                         // seven bits of fraction: no room for a value shifted by four
-                w[r][1] = H::fma(pick(lo >> 4, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
-                w[r][3] = H::fma(pick(lo >> 12, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
-              } else {                                             // 1024 + 16 q, times 1/16
-                w[r][1] = H::fma(pick(lo, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[r]);
-                w[r][3] = H::fma(pick(hi, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[r]);
-              }
-            }
-#pragma unroll
-            for (int b = 0; b < kNT; ++b) {
-              if ((q & kMask) == 0) H::mma0(part[b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
-              else H::mma(part[b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
-              H::mma(part[b], w[0][2], w[1][2], w[0][3], w[1][3], x[b].z, x[b].w);
-            }
-            if ((q & kMask) == kMask)
-#pragma unroll
-              for (int b = 0; b < kNT; ++b)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[b][c] = fmaf(part[b][c], scale[c >> 1], acc[b][c]);
+          for (int r = 0; r < 2; ++r) {
+            const uint2 v = *reinterpret_cast<const uint2*>(scales + ((q >> kShift) * kWarpRows + r * 8) * 8);
+            scale[r] = __uint_as_float(v.x);
+            sub0[r] = v.y;
+            if (!kBf16) sub1[r] = H::fma(sub0[r], H::kOne, H::kStep);      // -(64 + z)
           }
         }
-        __syncwarp();
-        ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->empty[stage]), lane);
-        advance();
+        uint4 x[kNT];
+#pragma unroll
+        for (int b = 0; b < kNT; ++b)
+          x[b] = *reinterpret_cast<const uint4*>(at + (x_first ^ ((q & 1) << 6)) + (quarter * 2 + (q >> 1)) * (kMp * 128) + b * 1024);
+        uint32_t w[2][4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t lo = *reinterpret_cast<const uint32_t*>(codes + (w_lane ^ (q << 4) ^ ((quarter & 1) << 6)) + r * 1024);
+          const uint32_t hi = lo >> 8;
+          w[r][0] = H::fma(pick(lo, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+          w[r][2] = H::fma(pick(hi, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+          if (kBf16) {                                                     // seven bits of fraction: no room for a value shifted by four
+            w[r][1] = H::fma(pick(lo >> 4, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+            w[r][3] = H::fma(pick(lo >> 12, 0x000f000fu, H::kMagic), H::kOne, sub0[r]);
+          } else {                                                         // 1024 + 16 q, times 1/16
+            w[r][1] = H::fma(pick(lo, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[r]);
+            w[r][3] = H::fma(pick(hi, 0x00f000f0u, H::kMagic), H::kSixteenth, sub1[r]);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kNT; ++b) {
+          if ((q & kMask) == 0) H::mma0(part[b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
+          else H::mma(part[b], w[0][0], w[1][0], w[0][1], w[1][1], x[b].x, x[b].y);
+          H::mma(part[b], w[0][2], w[1][2], w[0][3], w[1][3], x[b].z, x[b].w);
+        }
+        if ((q & kMask) == kMask)
+#pragma unroll
+          for (int b = 0; b < kNT; ++b)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[b][c] = fmaf(part[b][c], scale[c >> 1], acc[b][c]);
       }
-      if (!ok) break;
+    };
+    // sums of 16 rows as [part][activation row][weight row], once every stage has been read and the ring is free
+    auto keep = [&](const float (&acc)[kNT][4], int part, int unit) {
+      float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+      for (int b = 0; b < kNT; ++b)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          red[(part * kMp + b * 8 + t + 4 * (c & 1)) * p.rows + unit * 16 + g + 8 * (c >> 1)] = acc[b][c];
+    };
+    // x is ready: so are the codes, whose copies the x warps waited for
+    auto wait_stage = [&] {
+      return __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->ready[stage]), parity, abort_flag, p.wait_limit));
+    };
+    auto leave_stage = [&] {
+      __syncwarp();
+      ptx::mbar_arrive_lane0(ptx::smem_u32(&tail->empty[stage]), lane);
+      advance();
+    };
+    const int row = lane & 15;
+    if (warp < kWhole) {
+      const int unit = slices == 2 ? warp >> 1 : warp, slice = slices == 2 ? warp & 1 : 0;
+      float acc[kNT][4] = {};
+      if (unit < whole) {
+        const uint32_t area = kRing + warp * warp_area(kShift);
+        const int share = (lane >> 4) * kLaneGroups;                       // this lane's part of the scales: one half of a row's groups
+        ptx::griddep_wait();
+        RawScales<kLaneGroups> raw;
+        raw.load(p, n0 + unit * kWarpRows + row, step0 * kStepGroups + share);
+        bool ok = true;
+        for (int s0 = step0; s0 < step1 && ok; s0 += kSuper) {
+          __syncwarp();                                                    // the last scales have been read
+#pragma unroll
+          for (int j = 0; j < kLaneGroups; ++j)
+            *reinterpret_cast<uint2*>(smem + area + ((share + j) * kWarpRows + row) * 8) = raw.template ready<H>(j);
+          __syncwarp();
+          if (s0 + kSuper < step1) raw.load(p, n0 + unit * kWarpRows + row, (s0 + kSuper) * kStepGroups + share);
+          const int s1 = min(s0 + kSuper, step1);
+          for (int s = s0; s < s1; ++s) {
+            ok = wait_stage();
+            if (!ok) break;
+            const uint8_t* at = smem + stage * stage_bytes;
+            const uint8_t* scales = smem + area + ((s - s0) * kStepGroups * kWarpRows + g) * 8;
+            const uint8_t* codes = at + unit * 2048 + (slices == 2 ? slice * p.rows * 128 : 0);
+#pragma unroll
+            for (int piece = 0; piece < 4 / slices; ++piece) {
+              const int quarter = slices == 2 ? slice * 2 + piece : piece;
+              multiply(at, codes + (slices == 1 ? (piece >> 1) * p.rows * 128 : 0), scales + quarter * kPieceGroups * kWarpRows * 8, quarter, acc);
+            }
+            leave_stage();
+          }
+        }
+      }
+      named_sync(1, kThreads);
+      if (unit < whole) keep(acc, slice, unit);
+    } else if constexpr (kRest) {
+      const int quarter = warp - kWhole;
+      float acc[kRestUnits][kNT][4] = {};
+      if (rest > 0) {
+        const uint32_t area = kRing + kWhole * warp_area(kShift) + quarter * rest_area(kShift);
+        const int first = whole + (lane >> 4);                             // a lane's scales: its row of every other unit
+        RawScales<kPieceGroups> raw[(kRestUnits + 1) / 2];
+        auto load = [&](int s) {
+#pragma unroll
+          for (int i = 0; i < (kRestUnits + 1) / 2; ++i)
+            if (first + 2 * i < units) raw[i].load(p, n0 + (first + 2 * i) * kWarpRows + row, s * kStepGroups + quarter * kPieceGroups);
+        };
+        ptx::griddep_wait();
+        load(step0);
+        for (int s = step0; s < step1; ++s) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < (kRestUnits + 1) / 2; ++i)
+            if (first + 2 * i < units)
+#pragma unroll
+              for (int j = 0; j < kPieceGroups; ++j)
+                *reinterpret_cast<uint2*>(smem + area + (((first - whole + 2 * i) * kPieceGroups + j) * kWarpRows + row) * 8) =
+                    raw[i].template ready<H>(j);
+          __syncwarp();
+          if (s + 1 < step1) load(s + 1);
+          if (!wait_stage()) break;
+          const uint8_t* at = smem + stage * stage_bytes;
+          const uint8_t* codes = at + (quarter >> 1) * p.rows * 128 + whole * 2048;
+#pragma unroll
+          for (int i = 0; i < kRestUnits; ++i)
+            if (i < rest) multiply(at, codes + i * 2048, smem + area + (i * kPieceGroups * kWarpRows + g) * 8, quarter, acc[i]);
+          leave_stage();
+        }
+      }
+      named_sync(1, kThreads);
+#pragma unroll
+      for (int i = 0; i < kRestUnits; ++i)
+        if (i < rest) keep(acc[i], quarter, whole + i);
     }
   }
 
-  // ------------------------------------------------------------------ sums of the slices, then of the cluster's CTAs
-  __syncthreads();                                                 // every stage has been read: the ring is free
-  float* red = reinterpret_cast<float*>(smem);                     // [slice][activation row][weight row]
-  const int width = p.rows;
-  if (warp < kConsumers && slice < slices) {
-#pragma unroll
-    for (int b = 0; b < kNT; ++b)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        red[(slice * kMp + b * 8 + t + 4 * (c & 1)) * width + unit * 16 + g + 8 * (c >> 1)] = acc[b][c];
-  }
+  // ------------------------------------------------------------------ sums of the warps, then of the cluster's CTAs
+  if (warp >= kConsumers) named_sync(1, kThreads);                 // every stage has been read
   __syncthreads();
-  const bool whole = *abort_flag == 0;
+  float* red = reinterpret_cast<float*>(smem);
+  const int width = p.rows;
+  const bool done = *abort_flag == 0;
   const int count = min(kMp, p.m - m0) * width;
+  auto sum_of = [&](int i, int n) {
+    const int q = kMp * width;
+    float v = red[i];
+    if (kRest && n >= whole * kWarpRows) v += (red[q + i] + red[2 * q + i]) + red[3 * q + i];
+    else if (slices == 2) v += red[q + i];
+    return v;
+  };
+  auto split = [&](int i, int& m, int& n) {
+    m = static_cast<int>(__umulhi(static_cast<uint32_t>(i), p.row_share));
+    n = i - m * width;
+  };
   if (p.cluster > 1) {
     for (int i = threadIdx.x; i < count; i += kThreads) {
-      float v = red[i];
-      for (int s = 1; s < slices; ++s) v += red[s * kMp * width + i];
-      red[i] = v;
+      int m, n;
+      split(i, m, n);
+      red[i] = sum_of(i, n);
     }
     ptx::cluster_sync_all();
   }
-  auto store = [&](int i, float v) {
-    const int m = i / width, n = n0 + i - m * width;
+  auto store = [&](int m, int n, float v) {
+    n += n0;
     if (n >= p.n) return;
     if (p.bias != nullptr) v += __ldg(p.bias + n);
     const int64_t at = static_cast<int64_t>(m0 + m) * p.ldo + n;
@@ -396,17 +487,22 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   if (p.cluster > 1) {
     // CTA `rank` finishes its share of the outputs, adding the CTAs' sums in rank order, which is K order
     const int i1 = static_cast<int>(static_cast<long long>(count) * (rank + 1) / p.cluster);
-    for (int i = static_cast<int>(static_cast<long long>(count) * rank / p.cluster) + threadIdx.x; i < i1 && whole; i += kThreads) {
-      float v = 0.0f;
-      for (int c = 0; c < p.cluster; ++c) v += ld_cluster_f32(ptx::cluster_map(smem_base + i * 4, c));
-      store(i, v);
+    for (int i = static_cast<int>(static_cast<long long>(count) * rank / p.cluster) + threadIdx.x; i < i1 && done; i += kThreads) {
+      float part[kMaxCluster], v = 0.0f;                           // on their way together
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) part[c] = c < p.cluster ? ld_cluster_f32(ptx::cluster_map(smem_base + i * 4, c)) : 0.0f;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) v += part[c];
+      int m, n;
+      split(i, m, n);
+      store(m, n, v);
     }
     ptx::cluster_sync_all();                                       // nobody leaves while its sums are being read
-  } else if (whole) {
+  } else if (done) {
     for (int i = threadIdx.x; i < count; i += kThreads) {
-      float v = red[i];
-      for (int s = 1; s < slices; ++s) v += red[s * kMp * width + i];
-      store(i, v);
+      int m, n;
+      split(i, m, n);
+      store(m, n, sum_of(i, n));
     }
   }
   ptx::idle_after_abort(abort_flag);
@@ -419,47 +515,68 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 // that, a wave of CTAs 1.5 us to start and a cluster 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with
 // clusters of four, 7.2 us without; 1 row x 1024 x 1024: 3.0 us without, 4.4 us with pairs).  resident(c): clusters of c CTAs
 // that the device holds at once - 74 of two, but 33 of four and 15 of eight on 148 SMs.
+// A rest's warps count for the share of a whole warp's work that they have, and cost 0.3 us.
 struct Plan {
-  int rows, cluster;
+  int rows, cluster, slices;
+  bool rest;
 };
 template <typename Resident>
 Plan w4_plan(int64_t n, int64_t k, int64_t chunks, int nt, Resident resident) {
   const int64_t steps = (k + kStageK - 1) / kStageK;
-  const int most = 16 * consumers(nt) < kMaxRows ? 16 * consumers(nt) : kMaxRows;
-  Plan best = {16, 1};
-  constexpr int64_t kRate[2][4] = {{35, 66, 85, 100}, {30, 53, 65, 75}};         // bytes per 0.01 us
+  Plan best = {16, 1, 1, false};
+  constexpr int64_t kRate[2][5] = {{0, 35, 66, 85, 100}, {0, 30, 53, 65, 75}};   // bytes per 0.01 us
+  const int64_t* rates = kRate[nt - 1];
   int64_t best_cost = INT64_MAX;
   for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2) {
     if (cluster > steps) break;
     const int64_t together = resident(cluster);
     if (together <= 0) continue;
-    for (int rows = 16; rows <= most; rows += 16) {
-      const int64_t waves = ((n + rows - 1) / rows * chunks + together - 1) / together;
-      const int units = rows / 16, warps = 2 * units <= consumers(nt) ? 2 * units : units, most_warps = (warps + 3) / 4;
-      const int64_t each = (steps + cluster - 1) / cluster, codes = rows * each * 256 / warps * most_warps;
-      const int64_t cost = waves * (codes / kRate[nt - 1][most_warps - 1] + each * 15 + 150 + (cluster > 1 ? 120 : 0));
-      if (cost < best_cost || (cost == best_cost && cluster > best.cluster)) { best_cost = cost; best = {rows, cluster}; }
+    const int64_t each = (steps + cluster - 1) / cluster;
+    for (int units = 1; units <= kMaxRows / 16; ++units) {
+      const int64_t waves = ((n + units * 16 - 1) / (units * 16) * chunks + together - 1) / together;
+      for (int form = 0; form < 2; ++form) {
+        const bool rest = form != 0;
+        const int slices = 2 * whole_units(units, 2, rest) <= whole_warps(nt, rest) ? 2 : 1;
+        const int whole = whole_units(units, slices, rest), warps = (whole * slices + 3) / 4, more = (units - whole) * slices;
+        if (whole * slices > whole_warps(nt, rest) || rest != (more > 0)) continue;
+        // of the scheduler that has most: bytes of codes, and how fast its warps take them
+        const int64_t codes = each * 1024 * (rest ? units : 4 / slices * warps);
+        const int64_t rate = rates[warps] + (more > 0 ? (rates[warps + 1] - rates[warps]) * more / 4 : 0);
+        const int64_t cost = waves * (codes / rate + each * 15 + 150 + (cluster > 1 ? 120 : 0) + (rest ? 30 : 0));
+        if (cost < best_cost || (cost == best_cost && cluster > best.cluster)) {
+          best_cost = cost;
+          best = {units * 16, cluster, slices, rest};
+        }
+      }
     }
   }
   return best;
 }
 
+template <bool kBf16, int kNT, int kShift, int kSlices, bool kRest>
+int launch_form(cudaLaunchConfig_t& cfg, const CUtensorMap& tmap_w, const CUtensorMap& tmap_x, W4Params& p) {
+  constexpr int kRing = ring_bytes(kNT, kShift, kRest);
+  constexpr int smem = 1024 + kRing + scale_bytes(kNT, kShift, kRest) + static_cast<int>(sizeof(W4Tail));
+  static_assert(smem <= kSmemLimit, "shared memory of one SM");
+  static_assert(kRing / stage_size(kRest ? kMaxRows : 16 * whole_warps(kNT, false), kNT * 8) >= 2, "two stages at least");
+  static_assert(4 * kNT * 8 * kMaxRows * 4 <= kRing, "the warps' sums");
+  auto kernel = w4_kernel<kBf16, kNT, kShift, kSlices, kRest>;
+  static DeviceFlags done;
+  const int rc = ensure_smem_limit(kernel, kSmemLimit, done);
+  if (rc != BFP8_OK) return rc;
+  const int most = kRing / stage_size(p.rows, kNT * 8);
+  p.stages = most < kMaxStages ? most : kMaxStages;
+  cfg.blockDim = dim3(threads_of(kNT, kRest), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmap_w, tmap_x, p));
+  return BFP8_OK;
+}
+
 template <bool kBf16, int kNT, int kShift>
 int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  constexpr int kRing = ring_bytes(kNT, kShift);
-  constexpr int smem = 1024 + kRing + consumers(kNT) * warp_area(kShift) + static_cast<int>(sizeof(W4Tail));
   constexpr int kLaneGroups = super_steps(kShift) * step_groups(kShift) / 2;
-  static_assert(smem <= 227 * 1024, "shared memory of one SM");
   static_assert(kLaneGroups == 4 || kLaneGroups == 8, "what RawScales loads at once");
-  static_assert(kRing / stage_size(kMaxRows, kNT * 8) >= 2, "two stages at least");
-  auto whole = w4_kernel<kBf16, kNT, kShift, 1>, halves = w4_kernel<kBf16, kNT, kShift, 2>;
-  static DeviceFlags done_whole, done_halves;
-  int rc = ensure_smem_limit(whole, smem, done_whole);
-  if (rc == BFP8_OK) rc = ensure_smem_limit(halves, smem, done_halves);
-  if (rc != BFP8_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -472,21 +589,25 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   const int64_t chunks = (p.m + kNT * 8 - 1) / (kNT * 8);
   const Plan plan = w4_plan(p.n, p.k, chunks, kNT, [&](int cluster) -> int {
     if (cluster == 1) return sm_count();
+    // one CTA per SM in every form; asked for with the plain one
+    auto kernel = w4_kernel<kBf16, kNT, kShift, 1, false>;
+    static DeviceFlags done;
+    if (ensure_smem_limit(kernel, kSmemLimit, done) != BFP8_OK) return 0;
     cudaLaunchConfig_t ask = cfg;
     attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    ask.blockDim = dim3(threads_of(kNT, false), 1, 1);
+    ask.dynamicSmemBytes = 1024 + kSmemBytes;
     ask.gridDim = dim3(static_cast<unsigned>(cluster), 1, 1);
     ask.attrs = attr + 1;
     ask.numAttrs = 1;
-    return max_active_clusters(whole, ask, cluster, caps);
+    return max_active_clusters(kernel, ask, cluster, caps);
   });
   p.rows = plan.rows;
   p.cluster = plan.cluster;
+  p.row_share = 0xffffffffu / static_cast<uint32_t>(plan.rows) + 1u;
   p.scale_vec = p.groups % kLaneGroups == 0 && aligned(p.scales, 2 * kLaneGroups) && (p.zeros == nullptr || aligned(p.zeros, kLaneGroups));
-  const bool two = p.rows / 16 * 2 <= consumers(kNT);
-  const int most = kRing / stage_size(p.rows, kNT * 8);
-  p.stages = most < kMaxStages ? most : kMaxStages;
   alignas(64) CUtensorMap tmap_w, tmap_x;
-  rc = make_tensor_map_2d(&tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, p.k / 2, p.n, p.k / 2, 128, p.rows);
+  int rc = make_tensor_map_2d(&tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, p.k / 2, p.n, p.k / 2, 128, p.rows);
   if (rc != BFP8_OK) return rc;
   rc = make_tensor_map_2d(&tmap_x, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, p.k, p.m,
                           ldx * 2, 64, kNT * 8);
@@ -494,8 +615,11 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>(chunks), 1);
   attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
-  BFP8_CUDA_TRY(cudaLaunchKernelEx(&cfg, two ? halves : whole, tmap_w, tmap_x, p));
-  return BFP8_OK;
+  if (plan.rest)
+    return plan.slices == 2 ? launch_form<kBf16, kNT, kShift, 2, true>(cfg, tmap_w, tmap_x, p)
+                            : launch_form<kBf16, kNT, kShift, 1, true>(cfg, tmap_w, tmap_x, p);
+  return plan.slices == 2 ? launch_form<kBf16, kNT, kShift, 2, false>(cfg, tmap_w, tmap_x, p)
+                          : launch_form<kBf16, kNT, kShift, 1, false>(cfg, tmap_w, tmap_x, p);
 }
 
 template <bool kBf16, int kNT>

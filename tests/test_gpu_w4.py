@@ -60,6 +60,24 @@ def test_product_matches_the_definition(gk, m, n, k, group, dtype, zeros):
     _check(got, x, codes, scales, z, group)
 
 
+# On 148 SMs these leave groups of 16 rows over that four warps share: 5, 7, 9, 10, 13, 14 or 15 groups per CTA, with and
+# without clusters, the last CTA's rows and the last k ragged
+REST = [
+    (13, 9584, 1568), (9, 14213, 256), (13, 3184, 1568), (13, 19632, 544), (9, 21567, 544), (9, 4743, 3680), (9, 28585, 544),
+    (9, 30918, 256), (16, 3171, 3616), (1, 33201, 256), (13, 33345, 256), (16, 3374, 3776), (3, 7416, 3104), (8, 28719, 1056),
+]
+
+
+@pytest.mark.parametrize("group,dtype,zeros", [(32, torch.bfloat16, True), (64, torch.float16, True), (128, torch.bfloat16, False)])
+@pytest.mark.parametrize("m,n,k", REST)
+def test_rows_left_over(gk, m, n, k, group, dtype, zeros):
+    x, codes, scales, z = _problem(m, n, k, group, dtype, zeros)
+    x, codes, scales, z = _dev(x), _dev(codes), _dev(scales), _dev(z)
+    got = gk.gemm_group_w4(x, codes, scales, z, group=group, check=True)
+    _check(got.cpu(), x.cpu(), codes.cpu(), scales.cpu(), None if z is None else z.cpu(), group)
+    assert torch.equal(got, gk.gemm_group_w4(x, codes, scales, z, group=group))
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 77, 416), (11, 1000, 512), (40, 50, 288)])
 def test_fp32_output_and_bias(gk, m, n, k):
     x, codes, scales, z = _problem(m, n, k, 64, torch.bfloat16, True)
