@@ -147,7 +147,7 @@ __host__ __device__ constexpr int scale_bytes(int nt, int shift, bool rest) {
   return whole_warps(nt, rest) * warp_area(shift) + (rest ? 4 * rest_area(shift) : 0);
 }
 __host__ __device__ constexpr int ring_bytes(int nt, int shift, bool rest) { return (kSmemBytes - scale_bytes(nt, shift, rest)) & ~1023; }
-constexpr int64_t kMaxM = 65535 * 16;                      // activation rows: chunks of 16 on the grid's y axis
+constexpr int64_t kMaxM = 65535 * 16;                      // activation rows: chunks of 16 or more on the grid's y axis
 constexpr int kMaxRows = 16 * (whole_warps(1, true) + 3);                // weight rows per CTA, within a TMA box
 __host__ __device__ constexpr int stage_size(int rows, int mp) { return rows * (kStageK / 2) + mp * kStageK * 2; }
 
@@ -200,7 +200,7 @@ struct RawScales {
   }
 };
 
-// kNT: activation rows / 8; kShift: group = 32 << kShift; kSlices: warps that share 16 rows, 2 take a half of each stage's k
+// kNT: activation rows / 8, 1, 2 or 4; kShift: group = 32 << kShift; kSlices: warps that share 16 rows, 2 take a half of each stage's k
 // each; kRest: four more warps for the units left over.
 template <bool kBf16, int kNT, int kShift, int kSlices, bool kRest>
 __global__ void __launch_bounds__(threads_of(kNT, kRest), 1)
@@ -398,7 +398,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
             const uint8_t* at = smem + stage * stage_bytes;
             const uint8_t* scales = smem + area + ((s - s0) * kStepGroups * kWarpRows + g) * 8;
             const uint8_t* codes = at + unit * 2048 + (slices == 2 ? slice * p.rows * 128 : 0);
-#pragma unroll
+#pragma unroll(kNT == 4 ? 1 : 4)                           // with 32 rows the registers do not hold what four overlapping pieces need
             for (int piece = 0; piece < 4 / slices; ++piece) {
               const int quarter = slices == 2 ? slice * 2 + piece : piece;
               multiply(at, codes + (slices == 1 ? (piece >> 1) * p.rows * 128 : 0), scales + quarter * kPieceGroups * kWarpRows * 8, quarter, acc);
@@ -511,22 +511,22 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 
 // Rows per CTA and CTAs per cluster: the least time for the CTA that has most to do, priced with what B200 measured, in 0.01 us.
 // The SM's four schedulers have a quarter of the warps each, and the one with most of them sets the pace: one warp unpacks
-// 3.5 KB of codes per us, two 6.6, three 8.5 and four 10 (with 16 activation rows 3, 5.3, 6.5 and 7.5).  A stage costs 0.15 us beside
-// that, a wave of CTAs 1.5 us to start and a cluster 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with
+// 3.5 KB of codes per us, two 6.6, three 8.5 and four 10 (with 16 activation rows 3, 5.3, 6.5 and 7.5, with 32 rows 2.2, 4, 5 and 5.6).
+// A stage costs 0.15 us beside that, a wave of CTAs 1.5 us to start (with 32 rows 3.5 us after the first) and a cluster 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with
 // clusters of four, 7.2 us without; 1 row x 1024 x 1024: 3.0 us without, 4.4 us with pairs).  resident(c): clusters of c CTAs
 // that the device holds at once - 74 of two, but 33 of four and 15 of eight on 148 SMs.
 // A rest's warps count for the share of a whole warp's work that they have, and cost 0.3 us.
 struct Plan {
   int rows, cluster, slices;
   bool rest;
+  int64_t cost;
 };
 template <typename Resident>
 Plan w4_plan(int64_t n, int64_t k, int64_t chunks, int nt, Resident resident) {
   const int64_t steps = (k + kStageK - 1) / kStageK;
-  Plan best = {16, 1, 1, false};
-  constexpr int64_t kRate[2][5] = {{0, 35, 66, 85, 100}, {0, 30, 53, 65, 75}};   // bytes per 0.01 us
-  const int64_t* rates = kRate[nt - 1];
-  int64_t best_cost = INT64_MAX;
+  Plan best = {16, 1, 1, false, INT64_MAX};
+  constexpr int64_t kRate[3][5] = {{0, 35, 66, 85, 100}, {0, 30, 53, 65, 75}, {0, 22, 40, 50, 56}};   // bytes per 0.01 us
+  const int64_t* rates = kRate[nt / 2];
   for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2) {
     if (cluster > steps) break;
     const int64_t together = resident(cluster);
@@ -534,7 +534,7 @@ Plan w4_plan(int64_t n, int64_t k, int64_t chunks, int nt, Resident resident) {
     const int64_t each = (steps + cluster - 1) / cluster;
     for (int units = 1; units <= kMaxRows / 16; ++units) {
       const int64_t waves = ((n + units * 16 - 1) / (units * 16) * chunks + together - 1) / together;
-      for (int form = 0; form < 2; ++form) {
+      for (int form = 0; form < (nt == 4 ? 1 : 2); ++form) {
         const bool rest = form != 0;
         const int slices = 2 * whole_units(units, 2, rest) <= whole_warps(nt, rest) ? 2 : 1;
         const int whole = whole_units(units, slices, rest), warps = (whole * slices + 3) / 4, more = (units - whole) * slices;
@@ -542,11 +542,9 @@ Plan w4_plan(int64_t n, int64_t k, int64_t chunks, int nt, Resident resident) {
         // of the scheduler that has most: bytes of codes, and how fast its warps take them
         const int64_t codes = each * 1024 * (rest ? units : 4 / slices * warps);
         const int64_t rate = rates[warps] + (more > 0 ? (rates[warps + 1] - rates[warps]) * more / 4 : 0);
-        const int64_t cost = waves * (codes / rate + each * 15 + 150 + (cluster > 1 ? 120 : 0) + (rest ? 30 : 0));
-        if (cost < best_cost || (cost == best_cost && cluster > best.cluster)) {
-          best_cost = cost;
-          best = {units * 16, cluster, slices, rest};
-        }
+        const int64_t cost = waves * (codes / rate + each * 15 + 150 + (cluster > 1 ? 120 : 0) + (rest ? 30 : 0)) +
+                             (nt == 4 ? (waves - 1) * 200 : 0);
+        if (cost < best.cost || (cost == best.cost && cluster > best.cluster)) best = {units * 16, cluster, slices, rest, cost};
       }
     }
   }
@@ -572,28 +570,28 @@ int launch_form(cudaLaunchConfig_t& cfg, const CUtensorMap& tmap_w, const CUtens
   return BFP8_OK;
 }
 
-template <bool kBf16, int kNT, int kShift>
-int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  constexpr int kLaneGroups = super_steps(kShift) * step_groups(kShift) / 2;
-  static_assert(kLaneGroups == 4 || kLaneGroups == 8, "what RawScales loads at once");
+cudaLaunchConfig_t overlapped(cudaLaunchAttribute (&attr)[2], cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
-  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  attr[1].val.clusterDim = {1, 1, 1};
   cfg.attrs = attr;
-  static ClusterCaps caps;
-  const int64_t chunks = (p.m + kNT * 8 - 1) / (kNT * 8);
-  const Plan plan = w4_plan(p.n, p.k, chunks, kNT, [&](int cluster) -> int {
+  return cfg;
+}
+
+template <bool kBf16, int kNT, int kShift>
+Plan plan_for(const W4Params& p) {
+  return w4_plan(p.n, p.k, (p.m + kNT * 8 - 1) / (kNT * 8), kNT, [&](int cluster) -> int {
     if (cluster == 1) return sm_count();
     // one CTA per SM in every form; asked for with the plain one
     auto kernel = w4_kernel<kBf16, kNT, kShift, 1, false>;
     static DeviceFlags done;
+    static ClusterCaps caps;
     if (ensure_smem_limit(kernel, kSmemLimit, done) != BFP8_OK) return 0;
-    cudaLaunchConfig_t ask = cfg;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t ask = overlapped(attr, nullptr);
     attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
     ask.blockDim = dim3(threads_of(kNT, false), 1, 1);
     ask.dynamicSmemBytes = 1024 + kSmemBytes;
@@ -602,6 +600,14 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
     ask.numAttrs = 1;
     return max_active_clusters(kernel, ask, cluster, caps);
   });
+}
+
+template <bool kBf16, int kNT, int kShift>
+int launch_w4(const Plan& plan, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
+  constexpr int kLaneGroups = super_steps(kShift) * step_groups(kShift) / 2;
+  static_assert(kLaneGroups == 4 || kLaneGroups == 8, "what RawScales loads at once");
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = overlapped(attr, st);
   p.rows = plan.rows;
   p.cluster = plan.cluster;
   p.row_share = 0xffffffffu / static_cast<uint32_t>(plan.rows) + 1u;
@@ -612,29 +618,37 @@ int launch_w4(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cud
   rc = make_tensor_map_2d(&tmap_x, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, p.k, p.m,
                           ldx * 2, 64, kNT * 8);
   if (rc != BFP8_OK) return rc;
-  cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>(chunks), 1);
+  cfg.gridDim = dim3(static_cast<unsigned>((p.n + p.rows - 1) / p.rows * p.cluster), static_cast<unsigned>((p.m + kNT * 8 - 1) / (kNT * 8)), 1);
   attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
-  if (plan.rest)
-    return plan.slices == 2 ? launch_form<kBf16, kNT, kShift, 2, true>(cfg, tmap_w, tmap_x, p)
-                            : launch_form<kBf16, kNT, kShift, 1, true>(cfg, tmap_w, tmap_x, p);
+  if constexpr (kNT < 4)                                           // w4_plan knows no rest with 32 rows
+    if (plan.rest)
+      return plan.slices == 2 ? launch_form<kBf16, kNT, kShift, 2, true>(cfg, tmap_w, tmap_x, p)
+                              : launch_form<kBf16, kNT, kShift, 1, true>(cfg, tmap_w, tmap_x, p);
   return plan.slices == 2 ? launch_form<kBf16, kNT, kShift, 2, false>(cfg, tmap_w, tmap_x, p)
                           : launch_form<kBf16, kNT, kShift, 1, false>(cfg, tmap_w, tmap_x, p);
 }
 
-template <bool kBf16, int kNT>
-int launch_group(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  if (group == 32) return launch_w4<kBf16, kNT, 0>(codes, x, ldx, p, st);
-  if (group == 64) return launch_w4<kBf16, kNT, 1>(codes, x, ldx, p, st);
-  return launch_w4<kBf16, kNT, 2>(codes, x, ldx, p, st);
+// Up to 8 activation rows, 16, or more in several passes over the weight: of 32 rows where the price is no higher (the
+// prices of the two are good to a few percent) and they do not hold 16 rows of nothing, else of 16.  32 rows of bf16 in two
+// passes and in one: 4096 x 14336 22.0 and 20.2 us, 14336 x 4096 with groups of 64 23.5 and 20.5, 65536 x 1024 34.9 and 29.6,
+// but 28672 x 8192, which needs more groups of rows than eleven warps have, 73.6 and 83.3.
+template <bool kBf16, int kShift>
+int launch_rows(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
+  if (p.m <= 8) return launch_w4<kBf16, 1, kShift>(plan_for<kBf16, 1, kShift>(p), codes, x, ldx, p, st);
+  const Plan two = plan_for<kBf16, 2, kShift>(p);
+  if (p.m > 16 && (p.m + 31) / 32 * 32 - p.m < 16) {
+    const Plan four = plan_for<kBf16, 4, kShift>(p);
+    if (four.cost - two.cost <= two.cost / 50) return launch_w4<kBf16, 4, kShift>(four, codes, x, ldx, p, st);
+  }
+  return launch_w4<kBf16, 2, kShift>(two, codes, x, ldx, p, st);
 }
 
 template <bool kBf16>
-int launch_rows(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
-  // More than 16 rows in several passes over the weight: with the sums of 32 rows in its registers a warp spilled, and took
-  // 22.9 us for 32 x 4096 x 14336, 28.5 for 32 x 14336 x 4096 and 92 for 32 x 28672 x 8192 where two passes of 16 rows take
-  // 23.2, 24.1 and 77.
-  return p.m <= 8 ? launch_group<kBf16, 1>(group, codes, x, ldx, p, st) : launch_group<kBf16, 2>(group, codes, x, ldx, p, st);
+int launch_group(int group, const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
+  if (group == 32) return launch_rows<kBf16, 0>(codes, x, ldx, p, st);
+  if (group == 64) return launch_rows<kBf16, 1>(codes, x, ldx, p, st);
+  return launch_rows<kBf16, 2>(codes, x, ldx, p, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -716,7 +730,7 @@ extern "C" int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const
   p.wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kDefaultWaitLimit;
   p.status = status_dev;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return x_dtype == BFP8_W4_BF16 ? launch_rows<true>(group, codes, x, ldx, p, st) : launch_rows<false>(group, codes, x, ldx, p, st);
+  return x_dtype == BFP8_W4_BF16 ? launch_group<true>(group, codes, x, ldx, p, st) : launch_group<false>(group, codes, x, ldx, p, st);
 }
 
 extern "C" int bfp8_quant_group_w4_f32(const float* w, int64_t n, int64_t k, int64_t ldw, int group, uint8_t* codes,

@@ -50,7 +50,7 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
                   wait_limit_cycles=0):
     """[M, N] = x . W^T (+ bias), W[n, k] = (q[n, k] - z[n, k // group]) * scales[n, k // group].
 
-    x      bf16 or fp16 [M, K], K a multiple of 32; M <= 1048560, made for few rows (the weight is read once per 16)
+    x      bf16 or fp16 [M, K], K a multiple of 32; M <= 1048560, made for few rows (the weight is read once per 16 or 32)
     codes  uint8 [N, K / 2], q of even k in the low four bits;  scales of x's type [N, ceil(K / group)]
     zeros  uint8 of scales' shape, 0 .. 15, or None: 8;  bias fp32 [N] or None;  group 32, 64 or 128
     out    of x's type, or float32 with out_dtype=torch.float32; may not overlap x

@@ -384,7 +384,7 @@ int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* rout
  *   bias    fp32 [n] or NULL;  out of x's type, or fp32 with out_f32 != 0, [m, n], row stride ldo
  * group 32, 64 or 128, k a multiple of 32 (BFP8_ERR_UNSUPPORTED otherwise; the last group may be short).  q - z is exact,
  * sums are formed in fp32 in a fixed order, and a group's sum is multiplied by its scale in fp32.  Made for few rows: the
- * weight is read once per 16 of them; m <= 1048560.  A group's sum is formed before its scale is applied.  No workspace.  With bfp8_set_weights_at_rest the codes are requested before
+ * weight is read once per 16 or 32 of them; m <= 1048560.  A group's sum is formed before its scale is applied.  No workspace.  With bfp8_set_weights_at_rest the codes are requested before
  * the previous kernel of the stream has ended.  status |= WAIT_TIMEOUT if an internal wait gave up.  The reference has no
  * counterpart. */
 #define BFP8_W4_BF16 0

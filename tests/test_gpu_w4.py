@@ -78,6 +78,21 @@ def test_rows_left_over(gk, m, n, k, group, dtype, zeros):
     assert torch.equal(got, gk.gemm_group_w4(x, codes, scales, z, group=group))
 
 
+# Passes of 32 rows, full and short, of one and of two warps per 16 weight rows, with and without clusters
+MANY = [(32, 4100, 4096), (20, 9001, 1056), (31, 2065, 2080), (64, 4096, 1024), (57, 11003, 544), (17, 26001, 1056), (29, 5003, 3104)]
+
+
+@pytest.mark.parametrize("group,dtype,zeros", [(32, torch.float16, True), (64, torch.bfloat16, False), (128, torch.float16, True)])
+@pytest.mark.parametrize("m,n,k", MANY)
+def test_passes_of_32_rows(gk, m, n, k, group, dtype, zeros):
+    x, codes, scales, z = _problem(m, n, k, group, dtype, zeros)
+    x[m // 2, 3] = float("nan")                            # one row of a pass: the others do not see it
+    got = gk.gemm_group_w4(_dev(x), _dev(codes), _dev(scales), _dev(z), group=group, check=True).cpu()
+    assert torch.isnan(got[m // 2]).all()
+    keep = [r for r in range(m) if r != m // 2]
+    _check(got[keep], x[keep], codes, scales, z, group)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 77, 416), (11, 1000, 512), (40, 50, 288)])
 def test_fp32_output_and_bias(gk, m, n, k):
     x, codes, scales, z = _problem(m, n, k, 64, torch.bfloat16, True)
