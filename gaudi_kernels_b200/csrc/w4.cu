@@ -546,6 +546,7 @@ Plan w4_plan(int64_t n, int64_t k, int64_t chunks, int nt, Resident resident) {
                              (nt == 4 ? (waves - 1) * 200 : 0);
         if (cost < best.cost || (cost == best.cost && cluster > best.cluster)) best = {units * 16, cluster, slices, rest, cost};
       }
+      if (waves == 1) break;                                       // more rows per CTA only take longer
     }
   }
   return best;
