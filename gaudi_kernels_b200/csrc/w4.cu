@@ -11,16 +11,17 @@
 //   * which k a thread's operand register stands for is free as long as A and B agree: a thread owns 8 consecutive k of each
 //     32, the word as it lies in memory, and pairs (k, k + 4) of x by byte permutes.
 //   * the weight streams through a ring of shared-memory stages, 512 k of the CTA's rows each, by TMA; x comes with it, and one
-//     warp per 8 activation rows makes the permutes once for all others.  Scales and zero points go from global memory to
+//     warp per 8 activation rows (16 of 32) makes the permutes once for all others.  Scales and zero points go from global memory to
 //     the registers of the warp that has their rows, up to 1024 k ahead, and from there to its shared memory as fp32 scale
 //     and 16-bit offset.
 //   * a CTA has R rows (a multiple of 16) and a slice of K: R and the cluster size are chosen so that the CTAs fill the SMs
 //     once with the least per CTA (w4_plan).  Inside the CTA the warps split R and, where that leaves warps over, the k of
-//     a stage, evenly over the SM's schedulers; the CTAs of a cluster add their sums through distributed shared memory.  All sums in a fixed order.
-// Measured: 10.2 us for 1 x 14336 x 4096 (2.9 TB/s), 31 us for 8 x 28672 x 8192 with groups of 64 (4.1 TB/s).  The copies alone
-// take 7 and 19.6 us, the multiplication alone of resident data 9 and (with whole units
-// per warp only) 28: what bounds it is unpacking, 8 LOP3, 8
-// HFMA2 and 2 to 6 shifts per 512 weights and warp, in chains that three or four warps per scheduler do not hide.
+//     a stage, evenly over the SM's schedulers; the CTAs of a cluster add their sums through distributed shared memory.  All
+//     sums in a fixed order.
+// Measured: 10.3 us for 1 x 14336 x 4096 (2.9 TB/s), 31 us for 8 x 28672 x 8192 with groups of 64 (4.1 TB/s).  The copies alone
+// take 7 and 19.6 us; what bounds it is unpacking, 8 LOP3, 8 HFMA2 and 2 to 6 shifts per 512 weights and warp, in chains that
+// three or four warps per scheduler do not hide (the multiplication alone of resident data took 9 us, and 28 of 32 before
+// four warps shared the rows left over).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -130,10 +131,12 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // over four more warps take a piece each (8 x 28672 x 8192, 13 units: 32.4 us without, 31.1 with; 8 x 35520 x 8192, 15 units:
 // 50 us in two waves without, 36 with; 16 x 65536 x 1024: 21.1 and 18.6).  The rest's code costs 0.5 us where nothing is left.
 // (Quarters of a stage for all warps alike, which needs every unit's scales in reach of four warps: 36 us for 28672 x 8192.)
-__host__ __device__ constexpr int whole_warps(int nt, bool rest) { return rest ? 12 : 15 - nt; }
+// Beside them a warp per 8 rows of x and the producer; of 32 rows a warp has 16, which leaves 13 multiplying warps instead of
+// 11 and 28672 x 8192 in one wave: 58.7 us, not 83.
+__host__ __device__ constexpr int x_warps(int nt) { return nt < 4 ? nt : 2; }
+__host__ __device__ constexpr int whole_warps(int nt, bool rest) { return rest ? 12 : 15 - x_warps(nt); }
 __host__ __device__ constexpr int consumers(int nt, bool rest) { return whole_warps(nt, rest) + (rest ? 4 : 0); }
-// ... then one warp per 8 rows of x, and the producer
-__host__ __device__ constexpr int threads_of(int nt, bool rest) { return 32 * (consumers(nt, rest) + nt + 1); }
+__host__ __device__ constexpr int threads_of(int nt, bool rest) { return 32 * (consumers(nt, rest) + x_warps(nt) + 1); }
 __host__ __device__ constexpr int whole_units(int units, int slices, bool rest) {
   return !rest ? units : slices == 2 ? units & ~1 : min(units & ~3, whole_warps(1, true));
 }
@@ -206,7 +209,7 @@ template <bool kBf16, int kNT, int kShift, int kSlices, bool kRest>
 __global__ void __launch_bounds__(threads_of(kNT, kRest), 1)
 w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Params p) {
   using H = Half16<kBf16>;
-  constexpr int kWhole = whole_warps(kNT, kRest), kConsumers = consumers(kNT, kRest), kProducer = kConsumers + kNT;
+  constexpr int kWhole = whole_warps(kNT, kRest), kConsumers = consumers(kNT, kRest), kProducer = kConsumers + x_warps(kNT);
   constexpr int kWarpRows = 16, kThreads = threads_of(kNT, kRest), kRing = ring_bytes(kNT, kShift, kRest);
   constexpr int kMp = kNT * 8;
   constexpr int kXBytes = kMp * kStageK * 2;
@@ -234,7 +237,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       ptx::mbar_init(ptx::smem_u32(&tail->full[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&tail->ready[s]), kNT);
+      ptx::mbar_init(ptx::smem_u32(&tail->ready[s]), x_warps(kNT));
       ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), static_cast<uint32_t>(whole * slices + (rest > 0 ? 4 : 0)));
     }
     tail->abort_flag = 0;
@@ -283,18 +286,20 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     }
   } else if (warp >= kConsumers) {
     // ------------------------------------------------------------------ x of 8 rows: pairs (k, k + 4) side by side, once for all consumers
-    const uint32_t first = p.rows * 256 + ((warp - kConsumers) * 8 + xrow) * 128 + ((t ^ xrow) << 4);
+    constexpr int kEach = kNT / x_warps(kNT);
+    const uint32_t first = p.rows * 256 + ((warp - kConsumers) * kEach * 8 + xrow) * 128 + ((t ^ xrow) << 4);
     for (int s = step0; s < step1; ++s) {
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit))) break;
       uint8_t* at = smem + stage * stage_bytes;
 #pragma unroll
-      for (int h = 0; h < kStageK / 256; ++h) {
+      for (int h = 0; h < kEach * (kStageK / 256); ++h) {
+        uint8_t* half = at + (h / kEach) * 4 * (kMp * 128) + (h % kEach) * 1024;
         uint4 v[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const uint4*>(at + (first ^ ((q & 1) << 6)) + (h * 4 + (q >> 1)) * (kMp * 128));
+        for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const uint4*>(half + (first ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128));
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-          *reinterpret_cast<uint4*>(at + (first ^ ((q & 1) << 6)) + (h * 4 + (q >> 1)) * (kMp * 128)) =
+          *reinterpret_cast<uint4*>(half + (first ^ ((q & 1) << 6)) + (q >> 1) * (kMp * 128)) =
               make_uint4(__byte_perm(v[q].x, v[q].z, 0x5410), __byte_perm(v[q].x, v[q].z, 0x7632),
                          __byte_perm(v[q].y, v[q].w, 0x5410), __byte_perm(v[q].y, v[q].w, 0x7632));
       }
@@ -512,9 +517,10 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 // Rows per CTA and CTAs per cluster: the least time for the CTA that has most to do, priced with what B200 measured, in 0.01 us.
 // The SM's four schedulers have a quarter of the warps each, and the one with most of them sets the pace: one warp unpacks
 // 3.5 KB of codes per us, two 6.6, three 8.5 and four 10 (with 16 activation rows 3, 5.3, 6.5 and 7.5, with 32 rows 2.2, 4, 5 and 5.6).
-// A stage costs 0.15 us beside that, a wave of CTAs 1.5 us to start (with 32 rows 3.5 us after the first) and a cluster 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with
-// clusters of four, 7.2 us without; 1 row x 1024 x 1024: 3.0 us without, 4.4 us with pairs).  resident(c): clusters of c CTAs
-// that the device holds at once - 74 of two, but 33 of four and 15 of eight on 148 SMs.
+// A stage costs 0.15 us beside that, a wave of CTAs 1.5 us to start (with 32 rows 3.5 us after the first) and a cluster
+// 1.2 us to form and exchange its sums (3 rows x 1003 x 4000: 5.0 us with clusters of four, 7.2 us without; 1 row x 1024 x
+// 1024: 2.8 us without, 4.4 us with pairs).  resident(c): clusters of c CTAs that the device holds at once - 74 of two, but
+// 33 of four and 15 of eight on 148 SMs.
 // A rest's warps count for the share of a whole warp's work that they have, and cost 0.3 us.
 struct Plan {
   int rows, cluster, slices;
@@ -631,16 +637,17 @@ int launch_w4(const Plan& plan, const uint8_t* codes, const void* x, int64_t ldx
 }
 
 // Up to 8 activation rows, 16, or more in several passes over the weight: of 32 rows where the price is no higher (the
-// prices of the two are good to a few percent) and they do not hold 16 rows of nothing, else of 16.  32 rows of bf16 in two
-// passes and in one: 4096 x 14336 22.0 and 20.2 us, 14336 x 4096 with groups of 64 23.5 and 20.5, 65536 x 1024 34.9 and 29.6,
-// but 28672 x 8192, which needs more groups of rows than eleven warps have, 73.6 and 83.3.
+// prices of the two are good to a few percent), or a fifth lower where the passes would hold 16 rows of nothing; else of 16.
+// bf16 in passes of 16 and of 32: 32 rows, 4096 x 14336 22.0 and 20.1 us, 14336 x 4096 with groups of 64 23.5 and 20.8, 28672 x
+// 8192 73.5 and 58.7; 48 rows, 10240 x 8192 with groups of 32 52.5 and 60, 14336 x 4096 with groups of 64 42.7 and 33.
 template <bool kBf16, int kShift>
 int launch_rows(const uint8_t* codes, const void* x, int64_t ldx, W4Params& p, cudaStream_t st) {
   if (p.m <= 8) return launch_w4<kBf16, 1, kShift>(plan_for<kBf16, 1, kShift>(p), codes, x, ldx, p, st);
   const Plan two = plan_for<kBf16, 2, kShift>(p);
-  if (p.m > 16 && (p.m + 31) / 32 * 32 - p.m < 16) {
+  if (p.m > 16) {
     const Plan four = plan_for<kBf16, 4, kShift>(p);
-    if (four.cost - two.cost <= two.cost / 50) return launch_w4<kBf16, 4, kShift>(four, codes, x, ldx, p, st);
+    const bool filled = (p.m + 31) / 32 * 32 - p.m < 16;
+    if (four.cost - two.cost <= (filled ? two.cost / 50 : -two.cost / 5)) return launch_w4<kBf16, 4, kShift>(four, codes, x, ldx, p, st);
   }
   return launch_w4<kBf16, 2, kShift>(two, codes, x, ldx, p, st);
 }

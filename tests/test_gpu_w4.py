@@ -79,7 +79,8 @@ def test_rows_left_over(gk, m, n, k, group, dtype, zeros):
 
 
 # Passes of 32 rows, full and short, of one and of two warps per 16 weight rows, with and without clusters
-MANY = [(32, 4100, 4096), (20, 9001, 1056), (31, 2065, 2080), (64, 4096, 1024), (57, 11003, 544), (17, 26001, 1056), (29, 5003, 3104)]
+MANY = [(32, 4100, 4096), (20, 9001, 1056), (31, 2065, 2080), (64, 4096, 1024), (57, 11003, 544), (17, 26001, 1056), (29, 5003, 3104),
+        (33, 30777, 544), (47, 14336, 2048)]
 
 
 @pytest.mark.parametrize("group,dtype,zeros", [(32, torch.float16, True), (64, torch.bfloat16, False), (128, torch.float16, True)])
