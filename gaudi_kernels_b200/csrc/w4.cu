@@ -288,6 +288,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     // ------------------------------------------------------------------ x of 8 rows: pairs (k, k + 4) side by side, once for all consumers
     constexpr int kEach = kNT / x_warps(kNT);
     const uint32_t first = p.rows * 256 + ((warp - kConsumers) * kEach * 8 + xrow) * 128 + ((t ^ xrow) << 4);
+    ptx::griddep_wait();                                           // x comes only then: the previous kernel's time is not this wait's
     for (int s = step0; s < step1; ++s) {
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), parity, abort_flag, p.wait_limit))) break;
       uint8_t* at = smem + stage * stage_bytes;

@@ -55,7 +55,8 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
     zeros  uint8 of scales' shape, 0 .. 15, or None: 8;  bias fp32 [N] or None;  group 32, 64 or 128
     out    of x's type, or float32 with out_dtype=torch.float32; may not overlap x
     check  read the status word after the launch (one synchronisation) and raise if a bounded wait expired; status as in
-           gemm_block_fp8.  The kernel waits for nothing but its own copies, so calls are unchecked by default.
+           gemm_block_fp8.  The bounded waits are for the kernel's own copies, which begin when the previous kernel has
+           ended; CTAs of a cluster also wait for one another, each to its end.  So calls are unchecked by default.
     """
     kind = _DTYPE.get(x.dtype) if isinstance(x, torch.Tensor) else None
     if kind is None or x.ndim != 2 or not x.is_cuda or (x.stride(1) != 1 and x.shape[1] > 1):

@@ -201,6 +201,26 @@ def test_weights_at_rest_change_nothing(gk):
         gk.set_weights_at_rest(prev)
 
 
+@pytest.mark.parametrize("m,n", [(3, 1024), (20, 1024)])
+def test_the_previous_kernels_time_is_not_a_products_own_wait(gk, m, n):
+    # One row of 2^24 by 16 weight rows keeps at most eight SMs busy for milliseconds and lets its successor start at once on
+    # the others.  The product behind it may wait 100,000 cycles (about 50 us) for its own copies, which take a few.
+    long_k = 1 << 24
+    long_x = torch.zeros((1, long_k), dtype=torch.bfloat16, device=DEV)
+    long_codes = torch.zeros((16, long_k // 2), dtype=torch.uint8, device=DEV)
+    long_scales = torch.ones((16, long_k // 128), dtype=torch.bfloat16, device=DEV)
+    x, codes, scales, z = [_dev(v) for v in _problem(m, n, 1024, 64, torch.bfloat16, True)]
+    want = gk.gemm_group_w4(x, codes, scales, z, group=64, check=True)
+    for _ in range(3):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        gk.gemm_group_w4(long_x, long_codes, long_scales, group=128)
+        got = gk.gemm_group_w4(x, codes, scales, z, group=64, check=True, wait_limit_cycles=100000)
+        b.record()
+        b.synchronize()
+        assert torch.equal(got, want) and a.elapsed_time(b) > 0.3      # well beyond the limit: 100,000 cycles are 0.05 ms
+
+
 @pytest.mark.parametrize("scale_dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("zeros", [True, False])
 @pytest.mark.parametrize("n,k,group", [(1, 32, 32), (5, 96, 64), (33, 416, 128), (64, 1024, 32), (7, 160, 64)])
