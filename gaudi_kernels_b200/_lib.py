@@ -15,6 +15,7 @@ STATUS_BAD_INDEX = 0x10
 OUT_F32 = 0
 OUT_BF16 = 1
 SCHEDULE_FRESH_WEIGHT = 0x100
+W4_FRESH_CODES = 0x100
 
 _c = ctypes
 _i64, _ptr, _int, _sz, _f32 = _c.c_int64, _c.c_void_p, _c.c_int, _c.c_size_t, _c.c_float

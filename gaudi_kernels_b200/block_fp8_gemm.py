@@ -110,11 +110,12 @@ def new_status(device):
 
 
 def set_weights_at_rest(on):
-    """Tell the library whether the weight codes given to the decode-bucket GEMMs (M <= 128) are at rest, i.e. written
-    by nothing that is still in flight when a GEMM is enqueued (bfp8_set_weights_at_rest).  When they are, each GEMM
-    starts streaming its weight before the previous kernel of the stream has finished; results are unchanged.
+    """Tell the library whether the weight codes given to the decode-bucket GEMMs (M <= 128) and to gemm_group_w4 (any M)
+    are at rest, i.e. written by nothing that is still in flight when a GEMM is enqueued (bfp8_set_weights_at_rest).  When
+    they are, each GEMM starts streaming its weight before the previous kernel of the stream has finished; results are unchanged.
     Process-wide; returns the previous setting.  A serving process turns it on once its checkpoint is loaded and
-    the device synchronised, and off again around any in-place rewrite of a weight."""
+    the device synchronised, and off again around any in-place rewrite of a weight.  A call whose weight was written since
+    (by quantize_group_w4, say) is excepted by schedule=_lib.SCHEDULE_FRESH_WEIGHT or fresh_codes=True."""
     return bool(_lib.load().bfp8_set_weights_at_rest(1 if on else 0))
 
 

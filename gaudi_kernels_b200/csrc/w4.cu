@@ -717,6 +717,8 @@ extern "C" int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const
                                   const uint8_t* zeros, int group, const float* bias, void* out, int out_f32, int64_t ldo,
                                   int64_t m, int64_t n, int64_t k, uint32_t* status_dev, void* stream, int64_t wait_limit_cycles) {
   if (!x || !codes || !scales || !out || !status_dev) return BFP8_ERR_NULL;
+  const bool fresh_codes = (x_dtype & BFP8_W4_FRESH_CODES) != 0;
+  x_dtype &= ~BFP8_W4_FRESH_CODES;
   if (m <= 0 || n <= 0 || k <= 0 || m > kMaxM || n > (1 << 30) || k > (1 << 30) || ldx < k || ldo < n) return BFP8_ERR_SHAPE;
   if (x_dtype != BFP8_W4_BF16 && x_dtype != BFP8_W4_F16) return BFP8_ERR_SHAPE;
   if (group != 32 && group != 64 && group != 128) return BFP8_ERR_UNSUPPORTED;
@@ -735,7 +737,7 @@ extern "C" int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const
   p.k = static_cast<int>(k);
   p.groups = static_cast<int>((k + group - 1) / group);
   p.out_f32 = out_f32 != 0;
-  p.w_early = weights_at_rest() ? 1 : 0;
+  p.w_early = weights_at_rest() && !fresh_codes ? 1 : 0;
   p.wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kDefaultWaitLimit;
   p.status = status_dev;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

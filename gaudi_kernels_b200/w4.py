@@ -47,7 +47,7 @@ def quantize_group_w4(w, group=128, zeros=True, scale_dtype=torch.bfloat16):
 
 
 def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, out_dtype=None, check=False, status=None,
-                  wait_limit_cycles=0):
+                  wait_limit_cycles=0, fresh_codes=False):
     """[M, N] = x . W^T (+ bias), W[n, k] = (q[n, k] - z[n, k // group]) * scales[n, k // group].
 
     x      bf16 or fp16 [M, K], K a multiple of 32; M <= 1048560, made for few rows (the weight is read once per 16 or 32)
@@ -57,6 +57,8 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
     check  read the status word after the launch (one synchronisation) and raise if a bounded wait expired; status as in
            gemm_block_fp8.  The bounded waits are for the kernel's own copies, which begin when the previous kernel has
            ended; CTAs of a cluster also wait for one another, each to its end.  So calls are unchecked by default.
+    fresh_codes  the codes were written by a kernel enqueued just before this call (quantize_group_w4, a copy) and are not taken
+           to be at rest where set_weights_at_rest is on
     """
     kind = _DTYPE.get(x.dtype) if isinstance(x, torch.Tensor) else None
     if kind is None or x.ndim != 2 or not x.is_cuda or (x.stride(1) != 1 and x.shape[1] > 1):
@@ -97,7 +99,7 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
         if x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
             x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries, each its own
         st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
-        rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, kind, codes.data_ptr(),
+        rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, kind | (_lib.W4_FRESH_CODES if fresh_codes else 0), codes.data_ptr(),
                                     scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
                                     None if bias is None else bias.data_ptr(), out.data_ptr(),
                                     1 if out_dtype == torch.float32 else 0, out.stride(0) if m > 1 else n, m, n, k,

@@ -199,10 +199,11 @@ int bfp8_gemm_token_channel(const uint8_t* a_codes, int64_t lda, const float* a_
 int bfp8_gemm_k_split(int64_t m, int64_t n, int64_t k, int token_channel, int sms);
 
 /* Declares, for the whole process, whether the weight operands (w_codes) of the decode-bucket GEMMs (m <= 128:
- * bfp8_gemm_block128, _ex, _swiglu, _push, _noalloc) and of bfp8_gemm_group_w4 are at rest.  These kernels are launched so that their
- * set-up overlaps the end of the previous kernel of the stream, and normally touch no global memory until that
+ * bfp8_gemm_block128, _ex, _swiglu, _push, _noalloc) and the codes of bfp8_gemm_group_w4 (any m) are at rest.  These
+ * kernels are launched so that their set-up overlaps the end of the previous kernel of the stream, and normally touch no global memory until that
  * kernel has finished.  With on != 0 the caller promises that no work still in flight when such a GEMM is
- * enqueued writes its w_codes (weights were prepared at load time and the device was synchronised since); the
+ * enqueued writes its w_codes (weights were prepared at load time and the device was synchronised since; a call whose
+ * weight was written since carries BFP8_SCHEDULE_FRESH_WEIGHT or BFP8_W4_FRESH_CODES); the
  * kernel then requests the first weight tiles of every CTA before it waits for the previous kernel, so the
  * stream from HBM does not pause between the kernels of a decode step.  Activations, scales, bias, workspace
  * and output are still touched only after the wait, and results do not change.  Off by default; returns the
@@ -385,10 +386,12 @@ int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* rout
  * group 32, 64 or 128, k a multiple of 32 (BFP8_ERR_UNSUPPORTED otherwise; the last group may be short).  q - z is exact,
  * sums are formed in fp32 in a fixed order, and a group's sum is multiplied by its scale in fp32.  Made for few rows: the
  * weight is read once per 16 or 32 of them; m <= 1048560.  A group's sum is formed before its scale is applied.  No workspace.  With bfp8_set_weights_at_rest the codes are requested before
- * the previous kernel of the stream has ended.  status |= WAIT_TIMEOUT if an internal wait gave up.  The reference has no
+ * the previous kernel of the stream has ended, unless x_dtype | BFP8_W4_FRESH_CODES says that a kernel enqueued just before
+ * this call wrote them.  status |= WAIT_TIMEOUT if an internal wait gave up.  The reference has no
  * counterpart. */
 #define BFP8_W4_BF16 0
 #define BFP8_W4_F16  1
+#define BFP8_W4_FRESH_CODES 0x100         /* flag in the x_dtype argument */
 int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const uint8_t* codes, const uint16_t* scales,
                        const uint8_t* zeros, int group, const float* bias, void* out, int out_f32, int64_t ldo,
                        int64_t m, int64_t n, int64_t k, uint32_t* status_dev, void* stream, int64_t wait_limit_cycles);

@@ -201,6 +201,30 @@ def test_weights_at_rest_change_nothing(gk):
         gk.set_weights_at_rest(prev)
 
 
+def test_codes_written_just_before_the_product(gk):
+    # with weights at rest declared, codes that a kernel of the same stream has just written: one that lets its successor start
+    # early (the activation quantizer's bytes taken as codes) and the quantizer of the format
+    gen = torch.Generator().manual_seed(11)
+    x = _dev(torch.randn((4, 1024), generator=gen).to(torch.bfloat16))
+    rows = [_dev(torch.randn((4096, 512), generator=gen).to(torch.bfloat16)) for _ in range(3)]
+    scales = torch.ones((4096, 16), dtype=torch.bfloat16, device=DEV)
+    w = [_dev(torch.randn((4096, 1024), generator=gen)) for _ in range(3)]
+
+    def both(i):
+        codes = gk.quantize_act_1x128(rows[i])[0].view(torch.uint8)
+        y = gk.gemm_group_w4(x, codes, scales, group=64, fresh_codes=True)
+        codes, s, z = gk.quantize_group_w4(w[i], 64)
+        return y, gk.gemm_group_w4(x, codes, s, z, group=64, fresh_codes=True)
+
+    want = [both(i) for i in range(3)]
+    prev = gk.set_weights_at_rest(True)
+    try:
+        for n in range(12):
+            assert all(torch.equal(a, b) for a, b in zip(both(n % 3), want[n % 3]))
+    finally:
+        gk.set_weights_at_rest(prev)
+
+
 @pytest.mark.parametrize("m,n", [(3, 1024), (20, 1024)])
 def test_the_previous_kernels_time_is_not_a_products_own_wait(gk, m, n):
     # One row of 2^24 by 16 weight rows keeps at most eight SMs busy for milliseconds and lets its successor start at once on

@@ -112,6 +112,18 @@ def test_rows_and_strides_of_the_call(lib):                # noqa: F811
     assert args[1] == 136 and args[2] == 0 and args[6] == 64 and args[9] == 1 and args[10] == 50 and args[11:14] == (3, 40, 128)
 
 
+def test_fresh_codes_reach_the_call(lib, so):              # noqa: F811
+    import gaudi_kernels_b200 as gk
+    ops = _operands(dtype=torch.float16)
+    gk.gemm_group_w4(**ops)
+    gk.gemm_group_w4(**ops, fresh_codes=True)
+    assert [a[2] for a in lib.named("bfp8_gemm_group_w4")] == [1, 1 | 0x100]
+    args = [A, 64, 0x100, A, A, None, 64, None, A, 0, 16, 2, 16, 64, A + 1, None, 0]
+    assert so.bfp8_gemm_group_w4(*args) == -2              # the type under the flag is accepted: only the status word is misaligned
+    args[2] = 0x102
+    assert so.bfp8_gemm_group_w4(*args) == -3
+
+
 @pytest.mark.parametrize("m", [65535 * 16 + 1, 1 << 20])
 def test_more_rows_than_the_grid_holds(so, m):
     assert so.bfp8_gemm_group_w4(A, 64, 0, A, A, None, 64, None, A, 0, 16, m, 16, 64, A, None, 0) == -3
