@@ -188,88 +188,124 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int c, int h, bool v
   return v;
 }
 
-// A score decides which experts run, so its sum is held more exactly than fp32 would: products of bf16 numbers are exact in
-// fp32, 16 or 32 of them are added in fp32 from zero (off by a few parts in 10^8 of the score's spread) and these sums in
-// fp64, which B200 adds at half the fp32 rate.
+// A score decides which experts run, so its sum is formed in fp64: products of bf16 numbers are exact there, and the sum is off by
+// 2^-53 of its terms per addition.  (Sums of 16 or 32 terms in fp32 first, as the tensor core forms them, cost half the time for
+// many tokens, but put one of a hundred scores off by a step of fp32 where two columns of x are a thousand times the others, and
+// differ between batch sizes.  Both launches of the router, 1 x 64 x 2048, 8 x 256 x 4096, 128 x 256 x 4096: 4.2, 8.9 and 15.2 us,
+// with fp32 sums in blocks of 16 x 16 and a warp per token and expert 5.6, 8.0 and 9.8.)
 __device__ __forceinline__ float score_of(const FrontParams& p, double sum) {
   const float l = static_cast<float>(sum);
   return p.sigmoid ? static_cast<float>(1.0 / (1.0 + exp(-static_cast<double>(l)))) : l;
 }
 
-// Few tokens: one warp per token and expert.
-__device__ __forceinline__ void router_dot(const FrontParams& p, int64_t t, int e, int lane) {
-  double acc = 0.0;
-  const bool vec = p.vec != 0;
-  const uint16_t *xr = p.x + t * p.ldx, *wr = p.router + e * p.ldr;
-  for (int c = lane * 8; c < p.h; c += 512) {
-    float s = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint4 w = load8(wr, c + 256 * u, p.h, vec), v = load8(xr, c + 256 * u, p.h, vec);
-      const uint32_t *a = reinterpret_cast<const uint32_t*>(&w), *b = reinterpret_cast<const uint32_t*>(&v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s = fmaf(bf16_lo_to_float(a[j]), bf16_lo_to_float(b[j]), s);
-        s = fmaf(bf16_hi_to_float(a[j]), bf16_hi_to_float(b[j]), s);
-      }
-    }
-    acc += static_cast<double>(s);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane == 0) p.scores[t * p.experts + e] = score_of(p, acc);
+__device__ __forceinline__ double bf16_lo_to_double(uint32_t v) { return static_cast<double>(bf16_lo_to_float(v)); }
+__device__ __forceinline__ double bf16_hi_to_double(uint32_t v) { return static_cast<double>(bf16_hi_to_float(v)); }
+
+// c += a b, 8 rows x 4 k x 8 columns in fp64: lane 4 g + t has row g (column g) at one k of its choice and columns 2 t, 2 t + 1 of row g
+__device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
+  asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
 
-// More tokens: a block has 16 experts (the M dimension of mma.sync) and 8 kB tokens (N); its warps take turns in K, 32 at a
-// time, each product of 32 starting from zero.  A thread's operand registers are 8 consecutive k of its rows as they lie in
-// memory: which k a register stands for is free as long as both operands agree.  (128 tokens, 256 experts, H = 4096: plain
-// multiplications, each token's row read again for every two experts, took 46 us where this takes 7.)
-template <int kB>
+// Up to four tokens: eight warps per expert, each with every eighth 256 columns of its row, for all tokens.
+constexpr int kDotTokens = 4, kDotSlices = 8, kDotExperts = kFrontWarps / kDotSlices;
+__device__ __forceinline__ void router_dot(const FrontParams& p, int e0, int warp, int lane, double* red) {
+  double acc[kDotTokens] = {};
+  const bool vec = p.vec != 0;
+  const int e = e0 + warp / kDotSlices;
+  if (e < p.experts) {
+    const uint16_t* wr = p.router + e * p.ldr;
+#pragma unroll 2
+    for (int c = (warp % kDotSlices * 32 + lane) * 8; c < p.h; c += kDotSlices * 256) {
+      const uint4 w = load8(wr, c, p.h, vec);
+      uint4 x[kDotTokens];
+#pragma unroll
+      for (int t = 0; t < kDotTokens; ++t)
+        if (t < p.t) x[t] = load8(p.x + t * p.ldx, c, p.h, vec);
+      const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int t = 0; t < kDotTokens; ++t)
+        if (t < p.t) {
+          const uint32_t b[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc[t] = fma(bf16_lo_to_double(a[j]), bf16_lo_to_double(b[j]), acc[t]);
+            acc[t] = fma(bf16_hi_to_double(a[j]), bf16_hi_to_double(b[j]), acc[t]);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kDotTokens; ++t)
+    if (t < p.t) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
+      if (lane == 0) red[warp * kDotTokens + t] = acc[t];
+    }
+  __syncthreads();
+  const int i = threadIdx.x / kDotTokens, t = threadIdx.x % kDotTokens;
+  if (i < kDotExperts && e0 + i < p.experts && t < p.t) {
+    double v = 0.0;
+    for (int w = 0; w < kDotSlices; ++w) v += red[(i * kDotSlices + w) * kDotTokens + t];
+    p.scores[t * p.experts + e0 + i] = score_of(p, v);
+  }
+}
+
+// More tokens: a block has 8 kA experts (rows of the fp64 mma.sync) and 8 kB tokens (columns); its warps take turns in K, 32 at a
+// time.  A thread's operands are 8 consecutive k of its rows as they lie in memory: which k an operand stands for is free as long
+// as both agree.  fp64 bounds it, 64 multiplications per SM and cycle: 128 tokens, 256 experts and H = 4096 need 7.4 us, the kernel
+// takes 11.
+template <int kA, int kB>
 __device__ __forceinline__ void router_tile(const FrontParams& p, int64_t t0, int e0, double* red) {
+  constexpr int kE = 8 * kA, kT = 8 * kB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const bool vec = p.vec != 0;
-  double acc[kB][4];
-#pragma unroll
-  for (int b = 0; b < kB; ++b)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[b][c] = 0.0;
+  double acc[kA][kB][2] = {};
   const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-  const uint16_t *r0 = p.router + static_cast<int64_t>(e0 + g) * p.ldr, *r1 = r0 + 8 * p.ldr;
-  const bool has0 = e0 + g < p.experts, has1 = e0 + g + 8 < p.experts;
 #pragma unroll 4
   for (int c = warp * 32; c < p.h; c += kFrontWarps * 32) {
     const int k = c + t * 8;
-    const uint4 w0 = has0 ? load8(r0, k, p.h, vec) : none, w1 = has1 ? load8(r1, k, p.h, vec) : none;
-    uint4 x[kB];
+    uint4 w[kA], x[kB];
+#pragma unroll
+    for (int a = 0; a < kA; ++a) {
+      const int row = e0 + a * 8 + g;
+      w[a] = row < p.experts ? load8(p.router + row * p.ldr, k, p.h, vec) : none;
+    }
 #pragma unroll
     for (int b = 0; b < kB; ++b) {
       const int64_t row = t0 + b * 8 + g;
       x[b] = row < p.t ? load8(p.x + row * p.ldx, k, p.h, vec) : none;
     }
 #pragma unroll
-    for (int b = 0; b < kB; ++b) {
-      float s[4];
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-          : "=f"(s[0]), "=f"(s[1]), "=f"(s[2]), "=f"(s[3])
-          : "r"(w0.x), "r"(w1.x), "r"(w0.y), "r"(w1.y), "r"(x[b].x), "r"(x[b].y), "f"(0.0f));
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-          : "+f"(s[0]), "+f"(s[1]), "+f"(s[2]), "+f"(s[3]) : "r"(w0.z), "r"(w1.z), "r"(w0.w), "r"(w1.w), "r"(x[b].z), "r"(x[b].w));
+    for (int j = 0; j < 8; ++j) {
+      auto value = [&](const uint4& v) {
+        const uint32_t two = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+        return j & 1 ? bf16_hi_to_double(two) : bf16_lo_to_double(two);
+      };
+      double d[kB];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[b][j] += static_cast<double>(s[j]);
+      for (int b = 0; b < kB; ++b) d[b] = value(x[b]);
+#pragma unroll
+      for (int a = 0; a < kA; ++a) {
+        const double v = value(w[a]);
+#pragma unroll
+        for (int b = 0; b < kB; ++b) mma_f64(acc[a][b], v, d[b]);
+      }
     }
   }
   // the warps' sums, [warp][token][expert]
 #pragma unroll
-  for (int b = 0; b < kB; ++b)
+  for (int a = 0; a < kA; ++a)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) red[(warp * 8 * kB + b * 8 + 2 * t + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[b][j];
+    for (int b = 0; b < kB; ++b)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) red[(warp * kT + b * 8 + 2 * t + j) * kE + a * 8 + g] = acc[a][b][j];
   __syncthreads();
-  for (int i = threadIdx.x; i < 8 * kB * 16; i += kFrontWarps * 32) {
-    const int64_t token = t0 + i / 16;
-    const int e = e0 + i % 16;
+  for (int i = threadIdx.x; i < kT * kE; i += kFrontWarps * 32) {
+    const int64_t token = t0 + i / kE;
+    const int e = e0 + i % kE;
     if (token < p.t && e < p.experts) {
       double v = 0.0;
-      for (int w = 0; w < kFrontWarps; ++w) v += red[w * 8 * kB * 16 + i];
+      for (int w = 0; w < kFrontWarps; ++w) v += red[w * kT * kE + i];
       p.scores[token * p.experts + e] = score_of(p, v);
     }
   }
@@ -306,11 +342,11 @@ __device__ __forceinline__ void quantize_group(const FrontParams& p, int64_t t, 
   if (lane == 0) p.scales[static_cast<int64_t>(g) * p.t + t] = p.half ? scale * 2.0f : scale;
 }
 
-// kB: 8-token columns of a router block, 0: one warp per token and expert
-template <int kB>
+// kA, kB: a router block's experts and tokens / 8, 0: up to four tokens
+template <int kA, int kB>
 __global__ void __launch_bounds__(kFrontWarps * 32)
 moe_front_kernel(const FrontParams p) {
-  __shared__ double red[kB > 0 ? kFrontWarps * 8 * kB * 16 : 1];
+  __shared__ double red[kB > 0 ? kFrontWarps * 64 * kA * kB : kFrontWarps * kDotTokens];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -323,28 +359,29 @@ moe_front_kernel(const FrontParams p) {
   }
   const int64_t block = blockIdx.x - p.quant_blocks;
   if (kB == 0) {
-    const int64_t item = block * kFrontWarps + warp;
-    if (item < p.t * p.experts) router_dot(p, item / p.experts, static_cast<int>(item % p.experts), lane);
+    router_dot(p, static_cast<int>(block) * kDotExperts, warp, lane, red);
   } else {
-    const int eb = (p.experts + 15) / 16;
-    router_tile<kB == 0 ? 1 : kB>(p, block / eb * (8 * kB), static_cast<int>(block % eb) * 16, red);
+    const int eb = (p.experts + 8 * kA - 1) / (8 * kA);
+    router_tile<kA, kB == 0 ? 1 : kB>(p, block / eb * (8 * kB), static_cast<int>(block % eb) * (8 * kA), red);
   }
 }
 
 int launch_front(FrontParams& p, cudaStream_t st) {
   const int64_t quant = p.quant_blocks ? (p.t * p.groups + kFrontWarps - 1) / kFrontWarps : 0;
   p.quant_blocks = static_cast<int>(quant);
-  const int columns = p.t <= 4 ? 0 : p.t <= 8 ? 1 : 2;
+  // router blocks as small as lets the device hold them at once, one per SM
+  const int64_t e8 = (p.experts + 7) / 8, e16 = (p.experts + 15) / 16, t8 = (p.t + 7) / 8, t16 = (p.t + 15) / 16;
+  const int form = p.t <= kDotTokens ? 0 : e8 * t8 <= sm_count() ? 1 : e16 * t8 <= sm_count() ? 2 : 3;
   int64_t route = 0;
   if (p.router != nullptr)
-    route = columns == 0 ? (p.t * p.experts + kFrontWarps - 1) / kFrontWarps
-                         : (p.t + 8 * columns - 1) / (8 * columns) * ((p.experts + 15) / 16);
+    route = form == 0 ? (p.experts + kDotExperts - 1) / kDotExperts : form == 1 ? e8 * t8 : form == 2 ? e16 * t8 : e16 * t16;
   if (quant + route > 2147483647LL) return BFP8_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(quant + route)), block(kFrontWarps * 32);
-  switch (columns) {
-    case 0: return launch_overlapped(moe_front_kernel<0>, grid, block, 0, st, p);
-    case 1: return launch_overlapped(moe_front_kernel<1>, grid, block, 0, st, p);
-    default: return launch_overlapped(moe_front_kernel<2>, grid, block, 0, st, p);
+  switch (form) {
+    case 0: return launch_overlapped(moe_front_kernel<1, 0>, grid, block, 0, st, p);
+    case 1: return launch_overlapped(moe_front_kernel<1, 1>, grid, block, 0, st, p);
+    case 2: return launch_overlapped(moe_front_kernel<2, 1>, grid, block, 0, st, p);
+    default: return launch_overlapped(moe_front_kernel<2, 2>, grid, block, 0, st, p);
   }
 }
 

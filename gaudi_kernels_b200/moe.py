@@ -67,7 +67,7 @@ def _rows_apart(t, rows, width):
 def route_topk(x, router_weight, top_k, *, scoring="softmax", renormalize=True, bias=None, scale=1.0):
     """(ids int32 [T, top_k], weights fp32 [T, top_k]): the experts of every token, in descending order of their score.
 
-    l = fp32(x . router_weight^T) with the sum held to about 1e-8 of its terms' size.  scoring "softmax": the largest l,
+    l = fp32(x . router_weight^T), the sum formed in fp64.  scoring "softmax": the largest l,
     weights softmax(l) at them, over the chosen ones alone with `renormalize`.  "sigmoid": the largest
     fp32(sigmoid(l) + bias), weights sigmoid(l) at them, divided by their sum with `renormalize`.  Weights are multiplied by
     `scale`.  Ties go to the lower index; a NaN ranks last.  x bf16 [T, H], router_weight bf16 [E, H], E <= 512, any T.

@@ -331,7 +331,7 @@ int bfp8_peer_barrier(uint32_t* const* flags, int rank, int world_size, uint32_t
                       int64_t wait_limit_cycles, uint32_t* status_dev, void* stream);
 
 /* Router of a mixture-of-experts layer: the top_k experts of every token and their weights.
- *   l[t, e] = fp32(sum_c x[t, c] * router[e, c])          (the sum is held to about 1e-8 of its terms' size)
+ *   l[t, e] = fp32(sum_c x[t, c] * router[e, c])          (products exact, summed in fp64)
  *   BFP8_ROUTE_SOFTMAX  the largest l; weights softmax(l) at them (over the chosen ones alone with renormalize)
  *   BFP8_ROUTE_SIGMOID  s = fp32(sigmoid(l)); the largest fp32(s + bias) (bias may be NULL); weights s at them (divided
  *                       by their sum + 1e-20 with renormalize)

@@ -317,6 +317,40 @@ def test_route_matches_the_definition(gk, t, e, h, k, scoring, renorm):
     _check_route(got, (ids, w), gap, 2.5)
 
 
+@pytest.mark.parametrize("t,e,h", [(40, 250, 264), (40, 250, 77), (70, 500, 96), (6, 7, 2056), (200, 24, 40), (3, 511, 4104), (2, 1, 300)])
+def test_route_for_every_way_to_cut_the_work(gk, t, e, h):
+    x, r, bias = _route_problem(t, e, h)
+    k = min(e, 9)
+    want = moe_ref.route(x, r, k, "sigmoid", True, bias, 2.5)
+    _check_route(gk.route_topk(x.to(DEV), r.to(DEV), k, scoring="sigmoid", bias=bias.to(DEV), scale=2.5), want[:2], want[2], 2.5)
+
+
+@pytest.mark.parametrize("t", [1, 4, 5, 40, 300])
+def test_router_sums_are_exact_where_large_terms_cancel(gk, t):
+    # two columns of every token a thousand times the others, with products that cancel: what is left is the sum of the small
+    # terms, which fp32 sums lose to 2^-24 of the large ones
+    gen = torch.Generator().manual_seed(t)
+    e, h, k = 200, 2048, 8
+    x = torch.randn((t, h), generator=gen).to(torch.bfloat16)
+    r = (torch.randn((e, h), generator=gen) / h ** 0.5).to(torch.bfloat16)
+    x[:, 7] *= 1000
+    x[:, 1500] = -x[:, 7]
+    r[:, 1500] = r[:, 7]
+    l64 = x.double() @ r.double().t()
+    order = torch.sort(l64.float(), dim=1, descending=True, stable=True).indices[:, :k]
+    want = torch.sigmoid(l64.gather(1, order))
+    assert (l64.gather(1, order) > 0).all()
+    ids, w = gk.route_topk(x.to(DEV), r.to(DEV), k, scoring="sigmoid", renormalize=False)
+    # l and its sigmoid are rounded to fp32, half a step each: 2^-24 relative, the first times l (1 - sigmoid(l)) <= 0.28;
+    # sums of 2048 fp64 terms are off by 2048 2^-53 of their magnitudes' sum, about 200 here, which is far below
+    assert torch.equal(ids.cpu().long(), order)
+    assert ((w.double().cpu() - want).abs() <= 1.29 * 2.0 ** -24 * want).all()
+    # and no token's choice depends on how many others there are
+    for n in (1, 2, 5, 17):
+        part = gk.route_topk(x[:n].to(DEV), r.to(DEV), k, scoring="sigmoid", renormalize=False)
+        assert torch.equal(part[0], ids[:n]) and torch.equal(part[1], w[:n])
+
+
 def test_route_ties_go_to_the_lower_index(gk):
     x, r, _ = _route_problem(6, 40, 256)
     r[11], r[30], r[5] = r[2], r[2], r[39]
