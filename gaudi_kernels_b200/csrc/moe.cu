@@ -1049,7 +1049,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tmap_w13, const __grid_co
 
 // Layout of the workspace
 struct Layout {
-  size_t sync, x_codes, x_scales, scores, ids, weights, hq, h_scales, partials, y, bytes;
+  size_t sync, x_codes, x_scales, scores, hq, h_scales, partials, y, bytes;
   int spad;
 };
 Layout layout_of(int64_t t, int64_t k, int64_t e, int64_t h, int64_t i) {
@@ -1062,8 +1062,6 @@ Layout layout_of(int64_t t, int64_t k, int64_t e, int64_t h, int64_t i) {
   l.x_codes = take(static_cast<size_t>(t) * h);
   l.x_scales = take(static_cast<size_t>((h + 127) / 128) * t * 4);
   l.scores = take(static_cast<size_t>(t) * e * 4);
-  l.ids = take(static_cast<size_t>(slots) * 4);
-  l.weights = take(static_cast<size_t>(slots) * 4);
   l.hq = take(static_cast<size_t>(l.spad) * i);
   l.h_scales = take(static_cast<size_t>((i + 127) / 128) * l.spad * 4);
   l.partials = take(static_cast<size_t>(kMaxGrid) * 2 * 2 * (t <= 16 ? 16 : 64) * 128 * 4);
@@ -1153,8 +1151,8 @@ int moe_layer(const uint16_t* x, int64_t ldx, const Router* router, const int32_
   p.scores = f.scores;
   if (router) {
     p.rule = router->rule;
-    p.ids_out = ids_out ? ids_out : reinterpret_cast<int32_t*>(ws + l.ids);
-    p.weights = weights_out ? weights_out : reinterpret_cast<float*>(ws + l.weights);
+    p.ids_out = ids_out;
+    p.weights = weights_out;
   } else {
     p.ids = ids;
     p.weights = const_cast<float*>(weights);
