@@ -70,6 +70,8 @@ SIGNATURES = {
                                  _int, _ptr, _sz, _ptr, _ptr, _int, _i64]),
     "bfp8_moe_layer_block128": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _int, _int, _f32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
                                        _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _int, _ptr, _sz, _ptr, _ptr]),
+    "bfp8_moe_layer_block128_ex": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _int, _int, _f32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                          _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _int, _ptr, _sz, _ptr, _ptr, _int, _i64]),
 }
 
 _lib = None

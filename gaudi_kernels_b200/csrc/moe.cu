@@ -1247,17 +1247,29 @@ extern "C" int bfp8_moe_block128(const uint16_t* x, int64_t ldx, const int32_t* 
                    experts, h, inter, native_half, workspace, workspace_bytes, status_dev, stream, max_ctas, wait_limit_cycles);
 }
 
-extern "C" int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* router, int64_t ld_router, const float* bias,
-                                       int scoring, int renormalize, float scale, int32_t* ids, float* weights,
-                                       const uint8_t* w_gate_up, const float* s_gate_up, const uint8_t* w_down,
-                                       const float* s_down, uint16_t* out, int64_t ldo, int64_t t, int64_t top_k,
-                                       int64_t experts, int64_t h, int64_t inter, int native_half, void* workspace,
-                                       size_t workspace_bytes, uint32_t* status_dev, void* stream) {
+extern "C" int bfp8_moe_layer_block128_ex(const uint16_t* x, int64_t ldx, const uint16_t* router, int64_t ld_router,
+                                          const float* bias, int scoring, int renormalize, float scale, int32_t* ids,
+                                          float* weights, const uint8_t* w_gate_up, const float* s_gate_up, const uint8_t* w_down,
+                                          const float* s_down, uint16_t* out, int64_t ldo, int64_t t, int64_t top_k,
+                                          int64_t experts, int64_t h, int64_t inter, int native_half, void* workspace,
+                                          size_t workspace_bytes, uint32_t* status_dev, void* stream, int max_ctas,
+                                          int64_t wait_limit_cycles) {
   if (!router || !ids || !weights) return BFP8_ERR_NULL;
   if (scoring != BFP8_ROUTE_SOFTMAX && scoring != BFP8_ROUTE_SIGMOID) return BFP8_ERR_SHAPE;
   if (bias && scoring == BFP8_ROUTE_SOFTMAX) return BFP8_ERR_UNSUPPORTED;
   if (!aligned(router, 2) || (bias && !aligned(bias, 4)) || !aligned(ids, 4) || !aligned(weights, 4)) return BFP8_ERR_ALIGN;
   const Router r = {router, ld_router, {bias, scoring == BFP8_ROUTE_SOFTMAX, renormalize != 0, scale}, scoring == BFP8_ROUTE_SIGMOID};
   return moe_layer(x, ldx, &r, nullptr, nullptr, ids, weights, w_gate_up, s_gate_up, w_down, s_down, out, ldo, t, top_k, experts,
-                   h, inter, native_half, workspace, workspace_bytes, status_dev, stream, 0, 0);
+                   h, inter, native_half, workspace, workspace_bytes, status_dev, stream, max_ctas, wait_limit_cycles);
+}
+
+extern "C" int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* router, int64_t ld_router, const float* bias,
+                                       int scoring, int renormalize, float scale, int32_t* ids, float* weights,
+                                       const uint8_t* w_gate_up, const float* s_gate_up, const uint8_t* w_down,
+                                       const float* s_down, uint16_t* out, int64_t ldo, int64_t t, int64_t top_k,
+                                       int64_t experts, int64_t h, int64_t inter, int native_half, void* workspace,
+                                       size_t workspace_bytes, uint32_t* status_dev, void* stream) {
+  return bfp8_moe_layer_block128_ex(x, ldx, router, ld_router, bias, scoring, renormalize, scale, ids, weights, w_gate_up, s_gate_up,
+                                    w_down, s_down, out, ldo, t, top_k, experts, h, inter, native_half, workspace, workspace_bytes,
+                                    status_dev, stream, 0, 0);
 }

@@ -177,8 +177,12 @@ def moe_block_fp8(x, ids, weights, w_gate_up, s_gate_up, w_down, s_down, *, nati
 
 
 def moe_layer_block_fp8(x, router_weight, top_k, w_gate_up, s_gate_up, w_down, s_down, *, scoring="softmax", renormalize=True,
-                        bias=None, scale=1.0, native_half=False, out=None, check=True, status=None):
-    """(out bf16 [T, H], ids, weights): route_topk and moe_block_fp8 on its choice as two kernels, the same bits."""
+                        bias=None, scale=1.0, native_half=False, out=None, check=True, status=None, max_ctas=0,
+                        wait_limit_cycles=0):
+    """(out bf16 [T, H], ids, weights): route_topk and moe_block_fp8 on its choice as two kernels, the same bits.
+
+    Arguments as theirs; max_ctas and wait_limit_cycles are the experts' kernel's.
+    """
     _check_rows(x)
     t, h = x.shape
     dev = x.device
@@ -198,12 +202,13 @@ def moe_layer_block_fp8(x, router_weight, top_k, w_gate_up, s_gate_up, w_down, s
         nbytes = _workspace_bytes(t, top_k, experts, h, inter)
         ws = torch.empty_strided((nbytes,), (1,), dtype=_U8, device=dev)
         st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
-        rc = lib.bfp8_moe_layer_block128(x.data_ptr(), _row_stride(x, t, h), router_weight.data_ptr(),
-                                         _row_stride(router_weight, experts, h), None if bias is None else bias.data_ptr(),
-                                         _SCORING[scoring], 1 if renormalize else 0, scale, ids.data_ptr(), weights.data_ptr(),
-                                         w_gate_up.data_ptr(), s_gate_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(),
-                                         out.data_ptr(), _row_stride(out, t, h), t, top_k, experts, h, inter,
-                                         1 if native_half else 0, ws.data_ptr(), nbytes, st.data_ptr() + 8, _stream_ptr(dev))
+        rc = lib.bfp8_moe_layer_block128_ex(x.data_ptr(), _row_stride(x, t, h), router_weight.data_ptr(),
+                                            _row_stride(router_weight, experts, h), None if bias is None else bias.data_ptr(),
+                                            _SCORING[scoring], 1 if renormalize else 0, scale, ids.data_ptr(), weights.data_ptr(),
+                                            w_gate_up.data_ptr(), s_gate_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(),
+                                            out.data_ptr(), _row_stride(out, t, h), t, top_k, experts, h, inter,
+                                            1 if native_half else 0, ws.data_ptr(), nbytes, st.data_ptr() + 8, _stream_ptr(dev), max_ctas,
+                                            wait_limit_cycles)
         if rc:
             _lib.check(rc, "bfp8_moe_layer_block128")
         if check:

@@ -377,6 +377,15 @@ int bfp8_moe_layer_block128(const uint16_t* x, int64_t ldx, const uint16_t* rout
                             uint16_t* out, int64_t ldo, int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t inter,
                             int native_half, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream);
 
+/* The same with the controls of bfp8_moe_block128: at most max_ctas CTAs of the second kernel (0: one per SM), a limit on its
+ * internal waits (0: the default). */
+int bfp8_moe_layer_block128_ex(const uint16_t* x, int64_t ldx, const uint16_t* router, int64_t ld_router, const float* bias,
+                               int scoring, int renormalize, float scale, int32_t* ids, float* weights,
+                               const uint8_t* w_gate_up, const float* s_gate_up, const uint8_t* w_down, const float* s_down,
+                               uint16_t* out, int64_t ldo, int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t inter,
+                               int native_half, void* workspace, size_t workspace_bytes, uint32_t* status_dev, void* stream,
+                               int max_ctas, int64_t wait_limit_cycles);
+
 /* Product of a few activation rows with a 4-bit weight that has a scale (and a zero point) per group of k:
  *   out[i, j] = sum_k x[i, k] * (q[j, k] - z[j, k / group]) * s[j, k / group] (+ bias[j])
  *   x       bf16 (x_dtype BFP8_W4_BF16) or fp16 (BFP8_W4_F16) [m, k], row stride ldx (ldx % 8 == 0, 16-byte aligned)

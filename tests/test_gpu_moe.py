@@ -255,6 +255,27 @@ def test_an_expired_wait_is_reported_and_the_next_call_is_whole(gk):
     _check(_run(gk, args), args, False)
 
 
+@pytest.mark.parametrize("t", [2, 40])
+@pytest.mark.parametrize("ctas", [1, 7, 100])
+def test_the_layer_on_some_of_the_sms(gk, t, ctas):
+    x, _, _, *w = [a.to(DEV) for a in _problem(t, 3, 24, 272, 144)]
+    _, r, _ = _route_problem(1, 24, 272, seed=t)
+    ids, weights = gk.route_topk(x, r.to(DEV), 3)
+    want = gk.moe_block_fp8(x, ids, weights, *w, max_ctas=ctas)
+    out, i2, w2 = gk.moe_layer_block_fp8(x, r.to(DEV), 3, *w, max_ctas=ctas)
+    assert torch.equal(i2, ids) and torch.equal(w2, weights) and torch.equal(out, want)
+
+
+def test_an_expired_wait_of_the_layer_is_reported_and_the_next_call_is_whole(gk):
+    from gaudi_kernels_b200 import _lib
+    x, _, _, *w = [a.to(DEV) for a in _problem(9, 3, 4, 640, 528)]
+    _, r, _ = _route_problem(1, 4, 640)
+    want = gk.moe_layer_block_fp8(x, r.to(DEV), 3, *w)
+    with pytest.raises(_lib.Bfp8Error, match="bounded wait"):
+        gk.moe_layer_block_fp8(x, r.to(DEV), 3, *w, wait_limit_cycles=1)
+    assert all(torch.equal(a, b) for a, b in zip(gk.moe_layer_block_fp8(x, r.to(DEV), 3, *w), want))
+
+
 def test_experts_after_the_quantizer_and_the_gemm_of_one_stream(gk):
     # a decode step: a block-FP8 projection, the routed layer on its result, another projection - against the same calls
     # with a wait between them

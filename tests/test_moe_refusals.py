@@ -145,5 +145,15 @@ def test_strides_and_arguments_of_the_calls(lib):          # noqa: F811
     assert args[10:16] == (1, 2, 8, 256, 144, 1) and args[20] == 3
 
 
+def test_the_layer_takes_the_experts_controls(lib):        # noqa: F811
+    import gaudi_kernels_b200 as gk
+    ops = _operands()
+    router = torch.empty((8, 256), dtype=torch.bfloat16, device="cuda:0")
+    w = [ops[n] for n in ("w_gate_up", "s_gate_up", "w_down", "s_down")]
+    gk.moe_layer_block_fp8(ops["x"], router, 2, *w, check=False, max_ctas=100, wait_limit_cycles=7)
+    gk.moe_layer_block_fp8(ops["x"], router, 2, *w, check=False)
+    assert [a[-2:] for a in lib.named("bfp8_moe_layer_block128_ex")] == [(100, 7), (0, 0)]
+
+
 def test_misaligned_choices(so):
     assert _experts(so, ids=A + 2) == -2 and _experts(so, weights=A + 1) == -2
