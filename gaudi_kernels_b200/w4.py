@@ -46,6 +46,18 @@ def quantize_group_w4(w, group=128, zeros=True, scale_dtype=torch.bfloat16):
     return codes, scales, z
 
 
+def _share_memory(x, out):
+    """Whether matrices with unit column stride may have bytes in common (rows of one pitch are compared by their columns)."""
+    a, b = x.data_ptr(), out.data_ptr()
+    wide_a, wide_b = x.shape[1] * x.element_size(), out.shape[1] * out.element_size()
+    pitch_a, pitch_b = x.stride(0) * x.element_size(), out.stride(0) * out.element_size()
+    rows = x.shape[0]
+    if not a or not b or a + (rows - 1) * pitch_a + wide_a <= b or b + (rows - 1) * pitch_b + wide_b <= a:
+        return False                                       # apart, or without memory
+    off = (b - a) % pitch_a if rows > 1 and pitch_a == pitch_b else 0
+    return off < wide_a or off + wide_b > pitch_a
+
+
 def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, out_dtype=None, check=False, status=None,
                   wait_limit_cycles=0, fresh_codes=False):
     """[M, N] = x . W^T (+ bias), W[n, k] = (q[n, k] - z[n, k // group]) * scales[n, k // group].
@@ -53,7 +65,7 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
     x      bf16 or fp16 [M, K], K a multiple of 32; M <= 1048560, made for few rows (the weight is read once per 16 or 32)
     codes  uint8 [N, K / 2], q of even k in the low four bits;  scales of x's type [N, ceil(K / group)]
     zeros  uint8 of scales' shape, 0 .. 15, or None: 8;  bias fp32 [N] or None;  group 32, 64 or 128
-    out    of x's type, or float32 with out_dtype=torch.float32; may not overlap x
+    out    of x's type, or float32 with out_dtype=torch.float32; where it overlaps x, x is copied first
     check  read the status word after the launch (one synchronisation) and raise if a bounded wait expired; status as in
            gemm_block_fp8.  The bounded waits are for the kernel's own copies, which begin when the previous kernel has
            ended; CTAs of a cluster also wait for one another, each to its end.  So calls are unchecked by default.
@@ -92,12 +104,13 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
         raise ValueError("out must be [M, N] of out_dtype on x's device with unit column stride and rows apart")
     lib = _lib.load()
     with _device_guard(dev):
-        if out is None:
+        given = out is not None
+        if not given:
             out = _empty(m, n, out_dtype, dev)
         if m == 0:
             return out
-        if x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
-            x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries, each its own
+        if x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)) or (given and _share_memory(x, out)):
+            x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries, each its own, and reads on while outputs are stored
         st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
         rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, kind | (_lib.W4_FRESH_CODES if fresh_codes else 0), codes.data_ptr(),
                                     scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,

@@ -391,7 +391,8 @@ int bfp8_moe_layer_block128_ex(const uint16_t* x, int64_t ldx, const uint16_t* r
  *   x       bf16 (x_dtype BFP8_W4_BF16) or fp16 (BFP8_W4_F16) [m, k], row stride ldx (ldx % 8 == 0, 16-byte aligned)
  *   codes   uint8 [n, k / 2], contiguous, 16-byte aligned: q of even k in the low, of odd k in the high four bits
  *   scales  of x's type [n, ceil(k / group)], contiguous;  zeros uint8, the same shape, 0 .. 15, or NULL: 8
- *   bias    fp32 [n] or NULL;  out of x's type, or fp32 with out_f32 != 0, [m, n], row stride ldo
+ *   bias    fp32 [n] or NULL;  out of x's type, or fp32 with out_f32 != 0, [m, n], row stride ldo;
+ *           it may not overlap x
  * group 32, 64 or 128, k a multiple of 32 (BFP8_ERR_UNSUPPORTED otherwise; the last group may be short).  q - z is exact,
  * sums are formed in fp32 in a fixed order, and a group's sum is multiplied by its scale in fp32.  Made for few rows: the
  * weight is read once per 16 or 32 of them; m <= 1048560.  A group's sum is formed before its scale is applied.  No workspace.  With bfp8_set_weights_at_rest the codes are requested before

@@ -133,6 +133,20 @@ def test_strided_rows_and_a_given_output(gk):
     assert (big[0] == 3).all() and (big[6] == 3).all() and (big[:, :7] == 3).all() and (big[:, 137:] == 3).all()
 
 
+@pytest.mark.parametrize("m", [1, 5, 40])
+def test_an_output_over_the_rows_it_is_made_of(gk, m):
+    x, codes, scales, z = [_dev(v) for v in _problem(m, 4096, 4096, 128, torch.bfloat16, True)]
+    scales = scales * 0.01
+    want = gk.gemm_group_w4(x, codes, scales, z, group=128)
+    for _ in range(3):
+        y = x.clone()
+        assert gk.gemm_group_w4(y, codes, scales, z, group=128, out=y) is y and torch.equal(y, want)
+    wide = torch.zeros((m, 6144), dtype=torch.bfloat16, device=DEV)
+    wide[:, :4096] = x                                     # half of the output on x's columns, half beside them
+    gk.gemm_group_w4(wide[:, :4096], codes, scales, z, group=128, out=wide[:, 2048:])
+    assert torch.equal(wide[:, 2048:], want) and torch.equal(wide[:, :2048], x[:, :2048])
+
+
 def test_broadcast_rows(gk):
     x, codes, scales, z = _problem(5, 130, 256, 64, torch.bfloat16, True)
     same = _dev(x)[2:3].expand(5, 256)

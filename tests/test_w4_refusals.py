@@ -112,6 +112,31 @@ def test_rows_and_strides_of_the_call(lib):                # noqa: F811
     assert args[1] == 136 and args[2] == 0 and args[6] == 64 and args[9] == 1 and args[10] == 50 and args[11:14] == (3, 40, 128)
 
 
+def test_what_shares_memory():
+    from gaudi_kernels_b200.w4 import _share_memory
+    base = torch.empty((6, 64), dtype=torch.bfloat16)
+
+    def really(a, b):
+        def taken(t):
+            first = t.data_ptr()
+            return {first + 2 * (r * t.stride(0) + c) for r in range(t.shape[0]) for c in range(t.shape[1])}
+        return bool(taken(a) & taken(b))
+
+    views = [base[:3, :32], base[3:, :32], base[:3, 32:], base[1:4, 8:40], base[1:4, 40:64], base[:1, :32], base[2:3, 16:48],
+             base.view(12, 32)[:3], base.view(12, 32)[5:8, :16], base[:3, 31:63], base[:3]]
+    for a in views:
+        for b in views:
+            if a.shape[0] == b.shape[0]:
+                assert _share_memory(a, b) or not really(a, b)
+                if a.stride(0) == b.stride(0) and a.shape[0] > 1:          # rows of one pitch: exactly
+                    span = lambda t: (t.data_ptr(), t.data_ptr() + 2 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1]))    # noqa: E731
+                    apart = span(a)[1] <= span(b)[0] or span(b)[1] <= span(a)[0]
+                    columns = {(c + a.data_ptr() // 2) % a.stride(0) for c in range(a.shape[1])} & {
+                        (c + b.data_ptr() // 2) % b.stride(0) for c in range(b.shape[1])}
+                    assert _share_memory(a, b) == (bool(columns) and not apart)
+    assert not _share_memory(torch.empty((3, 8)), torch.empty((3, 8)))
+
+
 def test_fresh_codes_reach_the_call(lib, so):              # noqa: F811
     import gaudi_kernels_b200 as gk
     ops = _operands(dtype=torch.float16)
