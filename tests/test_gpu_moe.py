@@ -79,6 +79,22 @@ def test_experts_match_the_definition(gk, t, k, e, h, i, half):
     _check(_run(gk, args, native_half=half), args, half)
 
 
+# widths of real layers in one dimension at a time, and the widest allowed
+WIDE = [(1, 1, 2, 7168, 256), (3, 2, 4, 256, 14336), (20, 2, 3, 8192, 272), (20, 2, 3, 272, 8208), (1, 1, 1, 65536, 16), (18, 1, 2, 16, 65536)]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("t,k,e,h,i", WIDE)
+def test_wide_experts_match_the_definition(gk, t, k, e, h, i, half):
+    args = _problem(t, k, e, h, i)
+    got = _run(gk, args, native_half=half)
+    if max(h, i) < 65536:
+        _check(got, args, half)
+    else:                                                  # the bound of so long a sum is no longer small beside the result
+        y, bound = moe_ref.experts(*args, half)
+        assert ((got.double().cpu() - y).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("t,k", [(9, 3), (40, 2)])
 @pytest.mark.parametrize("ctas", [1, 2, 5, 31, 147])
 def test_any_number_of_ctas(gk, t, k, ctas):

@@ -215,6 +215,58 @@ def test_weights_at_rest_change_nothing(gk):
         gk.set_weights_at_rest(prev)
 
 
+@pytest.mark.parametrize("group,dtype,zeros", [(32, torch.bfloat16, True), (128, torch.float16, False)])
+@pytest.mark.parametrize("m,n", [(4, 1024), (4, 4096), (4, 33216), (13, 19648), (13, 33216), (32, 4096), (32, 28672), (40, 9600)])
+def test_products_at_rest_behind_products(gk, m, n, group, dtype, zeros):
+    # nothing but products in the stream, each launched over the end of the one whose result it reads: from 1024 columns to n and
+    # back, alone and in clusters, with rows left over and in passes of 32 rows; also replayed from a graph
+    up = [_dev(v) for v in _problem(m, n, 1024, group, dtype, zeros)]
+    down = [_dev(v) for v in _problem(m, 1024, n, group, dtype, zeros)]
+    up[2], down[2] = up[2] * 0.25, down[2] * 0.0625         # outputs stay in fp16's range
+    x = up[0]
+
+    def chain(wait):
+        y = x
+        for _ in range(4):
+            y = gk.gemm_group_w4(y, *up[1:], group=group)
+            if wait:
+                torch.cuda.synchronize()
+            y = gk.gemm_group_w4(y, *down[1:], group=group)
+            if wait:
+                torch.cuda.synchronize()
+        return y
+
+    want = chain(True)
+    assert torch.isfinite(want).all() and (want != 0).any()
+    prev = gk.set_weights_at_rest(True)
+    try:
+        torch.cuda.synchronize()
+        for _ in range(5):
+            assert torch.equal(chain(False), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = chain(False)
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    finally:
+        gk.set_weights_at_rest(prev)
+
+
+@pytest.mark.parametrize("group,dtype,zeros", [(32, torch.float16, True), (64, torch.bfloat16, False), (128, torch.bfloat16, True)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 28672), (5, 300, 20000), (8, 129, 65536), (12, 1003, 14336), (16, 90, 28672), (30, 500, 28672)])
+def test_long_rows(gk, m, n, k, group, dtype, zeros):
+    x, codes, scales, z = _problem(m, n, k, group, dtype, zeros)
+    scales = scales * 0.25                                 # fp16 outputs stay in range
+    got = gk.gemm_group_w4(_dev(x), _dev(codes), _dev(scales), _dev(z), group=group, check=True)
+    y, bound = w4_ref.product(x, codes, scales, z, group, None, dtype)
+    assert torch.isfinite(got).all() and ((got.double().cpu() - y).abs() <= bound).all()
+    # how small that bound is: 2048 + 26 additions at most, 2^-23 each of sum |terms|, and for terms of random signs
+    # sum |terms| is about sqrt(k) = 256 at most times |y|: 6.4 % beside the rounding of the output
+    assert float(bound.norm()) <= 0.07 * float(y.norm())
+
+
 def test_codes_written_just_before_the_product(gk):
     # with weights at rest declared, codes that a kernel of the same stream has just written: one that lets its successor start
     # early (the activation quantizer's bytes taken as codes) and the quantizer of the format
