@@ -19,8 +19,8 @@ def quantize_group_w4(w, group=128, zeros=True, scale_dtype=torch.bfloat16):
 
     With zeros: s = round((max(w, 0) - min(w, 0)) / 15), z = clamp(rne(-min / s), 0, 15); without: s = round(max|w| / 7) and
     z = 8 everywhere.  q = clamp(rne(w / s) + z, 0, 15).  Scales are rounded to scale_dtype (bfloat16 or float16) before they
-    are used.  K is a multiple of 32.  A group of zeros gets s = 1, one with a NaN s = NaN, one with an infinity (or a scale
-    beyond scale_dtype) s = inf: such a group does not read back as finite numbers.
+    are used.  K is a multiple of 32.  A group of zeros gets s = 1, one with a NaN s = NaN, one with an infinity (or a range
+    beyond fp32, or a scale beyond scale_dtype) s = inf: such a group does not read back as finite numbers.
     """
     if not isinstance(w, torch.Tensor) or w.dtype != torch.float32 or w.ndim != 2 or not w.numel() or w.stride(1) != 1:
         raise ValueError("expected a nonempty FP32 [N, K] tensor with unit stride along the last dimension")
@@ -62,7 +62,8 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
                   wait_limit_cycles=0, fresh_codes=False):
     """[M, N] = x . W^T (+ bias), W[n, k] = (q[n, k] - z[n, k // group]) * scales[n, k // group].
 
-    x      bf16 or fp16 [M, K], K a multiple of 32; M <= 1048560, made for few rows (the weight is read once per 16 or 32)
+    x      bf16 or fp16 [M, K], K a multiple of 32; M <= 1048560, made for few rows (the weight is read once per 16 or 32;
+           from about 32 rows on gemm_block_fp8 is faster)
     codes  uint8 [N, K / 2], q of even k in the low four bits;  scales of x's type [N, ceil(K / group)]
     zeros  uint8 of scales' shape, 0 .. 15, or None: 8;  bias fp32 [N] or None;  group 32, 64 or 128
     out    of x's type, or float32 with out_dtype=torch.float32; where it overlaps x, x is copied first

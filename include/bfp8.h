@@ -409,7 +409,7 @@ int bfp8_gemm_group_w4(const void* x, int64_t ldx, int x_dtype, const uint8_t* c
 /* fp32 weight [n, k] (row stride ldw) -> the codes, scales and zero points above.  zeros != NULL:
  * s = round16((max(w, 0) - min(w, 0)) / 15), z = clamp(rne(-min / s), 0, 15); zeros == NULL: s = round16(max|w| / 7),
  * z = 8.  q = clamp(rne(w / s) + z, 0, 15); a group of zeros, or one whose s rounds to zero, gets s = 1;
- * one with a NaN gets s = NaN, and one with an infinity, or whose s overflows the scale's type, s = inf: what it reads
+ * one with a NaN gets s = NaN, and one with an infinity, or whose range overflows fp32 or s the scale's type, s = inf: what it reads
  * back is then not finite. */
 int bfp8_quant_group_w4_f32(const float* w, int64_t n, int64_t k, int64_t ldw, int group, uint8_t* codes,
                             uint16_t* scales, uint8_t* zeros, int scale_dtype, void* stream);
