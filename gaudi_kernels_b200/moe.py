@@ -207,8 +207,8 @@ def moe_layer_block_fp8(x, router_weight, top_k, w_gate_up, s_gate_up, w_down, s
                                             _SCORING[scoring], 1 if renormalize else 0, scale, ids.data_ptr(), weights.data_ptr(),
                                             w_gate_up.data_ptr(), s_gate_up.data_ptr(), w_down.data_ptr(), s_down.data_ptr(),
                                             out.data_ptr(), _row_stride(out, t, h), t, top_k, experts, h, inter,
-                                            1 if native_half else 0, ws.data_ptr(), nbytes, st.data_ptr() + 8, _stream_ptr(dev), max_ctas,
-                                            wait_limit_cycles)
+                                            1 if native_half else 0, ws.data_ptr(), nbytes, st.data_ptr() + 8, _stream_ptr(dev),
+                                            max_ctas, wait_limit_cycles)
         if rc:
             _lib.check(rc, "bfp8_moe_layer_block128")
         if check:

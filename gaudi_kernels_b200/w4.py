@@ -111,9 +111,11 @@ def gemm_group_w4(x, codes, scales, zeros=None, *, group, bias=None, out=None, o
         if m == 0:
             return out
         if x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)) or (given and _share_memory(x, out)):
-            x = x.contiguous() if not x.is_contiguous() else x.clone()         # TMA reads rows from 16-byte boundaries, each its own, and reads on while outputs are stored
+            # TMA reads rows from 16-byte boundaries, each its own, and reads on while outputs are stored
+            x = x.contiguous() if not x.is_contiguous() else x.clone()
         st = status if status is not None else _status_buffer(dev) if check else _status_sink(dev)
-        rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k, kind | (_lib.W4_FRESH_CODES if fresh_codes else 0), codes.data_ptr(),
+        rc = lib.bfp8_gemm_group_w4(x.data_ptr(), x.stride(0) if m > 1 else k,
+                                    kind | (_lib.W4_FRESH_CODES if fresh_codes else 0), codes.data_ptr(),
                                     scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
                                     None if bias is None else bias.data_ptr(), out.data_ptr(),
                                     1 if out_dtype == torch.float32 else 0, out.stride(0) if m > 1 else n, m, n, k,

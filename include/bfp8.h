@@ -200,8 +200,8 @@ int bfp8_gemm_k_split(int64_t m, int64_t n, int64_t k, int token_channel, int sm
 
 /* Declares, for the whole process, whether the weight operands (w_codes) of the decode-bucket GEMMs (m <= 128:
  * bfp8_gemm_block128, _ex, _swiglu, _push, _noalloc) and the codes of bfp8_gemm_group_w4 (any m) are at rest.  These
- * kernels are launched so that their set-up overlaps the end of the previous kernel of the stream, and normally touch no global memory until that
- * kernel has finished.  With on != 0 the caller promises that no work still in flight when such a GEMM is
+ * kernels are launched so that their set-up overlaps the end of the previous kernel of the stream, and normally
+ * touch no global memory until that kernel has finished.  With on != 0 the caller promises that no work still in flight when such a GEMM is
  * enqueued writes its w_codes (weights were prepared at load time and the device was synchronised since; a call whose
  * weight was written since carries BFP8_SCHEDULE_FRESH_WEIGHT or BFP8_W4_FRESH_CODES); the
  * kernel then requests the first weight tiles of every CTA before it waits for the previous kernel, so the
